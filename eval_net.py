@@ -261,6 +261,9 @@ def main(argv=None):
     parser.add_argument("--graph", action="store_true", help="hipGraph replay per (lambda, shape)")
     parser.add_argument("--per-image", action="store_true", dest="per_image",
                         help="--synthetic-kodak: one image per forward instead of one batch per image shape")
+    parser.add_argument("--int8-linear", action="store_true", dest="int8_linear",
+                        help="the window-attention blocks' Linears in 8-bit integer products (a scale for each token "
+                             "and output channel); encoder and decoder have to agree on it")
     parser.add_argument("--gpus", type=int, default=1,
                         help="ranks (one per GPU); without torchrun this process starts them itself")
     args = parser.parse_args(argv)
@@ -274,6 +277,12 @@ def main(argv=None):
                                                                                  else list(argv)), args.gpus))
     if D.launched() and D.env_rank()[1] != args.gpus and args.gpus > 1:
         raise SystemExit(f"eval_net.py: --gpus {args.gpus} but the launcher started {D.env_rank()[1]} ranks")
+    from lic_amd.functional import int8_linears
+    with int8_linears(args.int8_linear):
+        evaluate(args)
+
+
+def evaluate(args):
     if args.synthetic_kodak:
         lambdas = [float(v) for v in args.lambdas.split(",") if v]
         prec = args.precision if args.precision_given else "fp32x6"
@@ -282,7 +291,8 @@ def main(argv=None):
         if int(os.environ.get("RANK", 0)) == 0:
             print(json.dumps({"metric": "images/sec encode+decode (Kodak-24 R-D sweep, 768x512)",
                               "value": round(ips, 2), "unit": "images/s", "n_gpus": world,
-                              "arch": args.arch, "precision": prec, "graph": args.graph,
+                              "arch": args.arch, "precision": prec + ("+int8_linear" if args.int8_linear else ""),
+                              "graph": args.graph,
                               "batching": "per image" if args.per_image else "one batch per (lambda, image shape)",
                               "data": "synthetic Kodak-shaped images, seeded weights per lambda",
                               "rd": summ}), flush=True)

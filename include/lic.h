@@ -591,16 +591,66 @@ typedef struct lic_wba16_args {
 } lic_wba16_args;
 int lic_wba16_qkv_attn_fwd(const lic_wba16_args* a, lic_stream_t stream);
 
+/* Rotary positions over several axes: y = x with `pairs` channel pairs of each of `heads` heads (head j:
+ * channels [j*head_dim, (j+1)*head_dim) of the view) rotated by t = pos[axis(p)] * freq(p):
+ *   (a, b) -> (a cos t - b sin t, a sin t + b cos t)       (inverse != 0: by -t, which is the gradient)
+ * layout LIC_ROTARY_HALF: pair p = channels (p, p + pairs) of the head; LIC_ROTARY_PAIRS: (2p, 2p + 1).
+ * Channels [2*pairs, head_dim) of a head and [heads*head_dim, c) of the view are copied (y == x: left).
+ * table: device, per pair {uint64 freq / 2pi in units of 2^-64 turns (mod 1), int32 axis, int32 0}.
+ * pos: int32 [naxes][n][h*w] (pos_per_image != 0) or [naxes][h*w], contiguous; NULL: the grid's own
+ * positions, naxes 1: y*w + x, 2: (y, x), 3: (image, y, x).  y == x (same ld) rotates in place; other
+ * overlaps are the caller's to avoid.  naxes <= LIC_ROTARY_MAX_AXES. */
+#define LIC_ROTARY_MAX_AXES 4
+enum lic_rotary_layout { LIC_ROTARY_HALF = 0, LIC_ROTARY_PAIRS = 1 };
+int lic_rotary(int32_t dtype, const void* x, int32_t ldx, int32_t n, int32_t h, int32_t w, int32_t c,
+               int32_t heads, int32_t head_dim, int32_t pairs, int32_t layout, const void* table,
+               int32_t naxes, const int32_t* pos, int32_t pos_per_image, int32_t inverse, void* y, int32_t ldy,
+               lic_stream_t stream);
+
+/* Products in 8-bit integers with a scale for each token (row of x) and output channel.
+ * lic_quantize_int8: codes[i][j] = rint(127 x[i][j] / max_j |x[i][j]|) (exact, half to even; zero for a
+ * zero row), scale[i] = max_j |x[i][j]| / 127, columns [k, kpad) zero; a row that holds a NaN or an infinity
+ * gets zero codes and a NaN scale, which makes its whole output row NaN.  Also packs weights (rows =
+ * output channels).  kpad: a multiple of 64, >= k; codes 16-byte aligned.
+ * lic_linear_int8: y[i][o] = act(xscale[i] * wscale[o] * sum_j xcodes[i][j] * w[o][j] + bias[o]) + r1[i][o],
+ * the sum in 32-bit integers (k <= 131072 cannot overflow), the rest in fp32, rounded once to `dtype`.
+ * Either xcodes / xscale ([m][kpad], fp32 [m]) or x (m rows of k, stride ldx, quantised by the call) is given.
+ * act: LIC_ACT_NONE / RELU / LRELU / GELU; bias and r1 may be NULL; y must not overlap x, xcodes or w (r1 may
+ * be y).  ws: lic_linear_int8_workspace bytes, 16-byte aligned (needed with x only; 0 with xcodes). */
+#define LIC_INT8_MAX_K 131072
+int lic_quantize_int8(int32_t dtype, const void* x, int64_t ldx, int32_t m, int32_t k, int8_t* codes, int32_t kpad,
+                      float* scale, lic_stream_t stream);
+int64_t lic_linear_int8_workspace(int32_t m, int32_t kpad);
+int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const int8_t* xcodes, const float* xscale, int32_t m,
+                    int32_t k, const int8_t* w, int32_t kpad, const float* wscale, const float* bias, int32_t n,
+                    int32_t act, float slope, const void* r1, int64_t ldr1, void* y, int64_t ldy, void* ws,
+                    int64_t ws_bytes, lic_stream_t stream);
+
+/* Newton-Schulz orthogonalisation of `count` matrices at once (the update of the Muon optimiser):
+ *   X = G / (|G|_F + eps);  `steps` times: A = X X^T, X = (a I + b A + c A A) X     (on G^T if rows > cols)
+ * g: `dtype` elements at g + i*rs + j*cs (any strides), out: rows x cols, contiguous, `dtype`.  `mats` is a
+ * host array (read before the call returns).  coeffs = {a, b, c}.  Deterministic (no atomics).
+ * ws: lic_orthogonalize_workspace bytes of device memory, 256-byte aligned, -1: sizes out of range. */
+typedef struct lic_ortho_mat {
+  const void* g; int64_t rs, cs;
+  void* out;
+  int32_t rows, cols;
+} lic_ortho_mat;
+int64_t lic_orthogonalize_workspace(int32_t dtype, int32_t count, const lic_ortho_mat* mats);
+int lic_orthogonalize(int32_t dtype, int32_t count, const lic_ortho_mat* mats, int32_t steps, const float* coeffs,
+                      float eps, void* ws, int64_t ws_bytes, lic_stream_t stream);
+
 /* Library info.
  * LIC_ABI_VERSION changes whenever an entry point's parameter list or an args struct's layout
  * changes (3: lic_conv_args.mfma_mode / wgt_split, lic_rate_train_* seed_dev / seed_mul; 5:
  * lic_resunit_args / lic_resunit_fwd; 6: lic_wba_args / lic_wba_qkv_attn_fwd; 7: lic_wba16_args /
- * lic_wba16_qkv_attn_fwd).  A
+ * lic_wba16_qkv_attn_fwd; 8: lic_ortho_mat / lic_orthogonalize, lic_rotary, lic_quantize_int8,
+ * lic_linear_int8).  A
  * caller compiled against this header checks lic_abi_version() == LIC_ABI_VERSION and
  * lic_args_size(k) == sizeof(...) once after loading the library (the Python host does, _ffi.load). */
-#define LIC_ABI_VERSION 7
+#define LIC_ABI_VERSION 8
 enum { LIC_ARGS_CONV = 0, LIC_ARGS_ATTN = 1, LIC_ARGS_RATE = 2, LIC_ARGS_RANS = 3, LIC_ARGS_WGRAD = 4,
-       LIC_ARGS_RESUNIT = 5, LIC_ARGS_WBA = 6, LIC_ARGS_WBA16 = 7 };
+       LIC_ARGS_RESUNIT = 5, LIC_ARGS_WBA = 6, LIC_ARGS_WBA16 = 7, LIC_ARGS_ORTHO = 8 };
 const char* lic_last_error(void);
 const char* lic_version(void);          /* "liblic <ver> gfx950 (abi N, src <source hash>)" */
 /* Build provenance: the first 16 hex digits of the SHA-256 of the sources the library was built

@@ -33,7 +33,7 @@ ACT_NONE, ACT_RELU, ACT_LRELU, ACT_GELU, ACT_ROUND = 0, 1, 2, 3, 4
 PRO_NONE, PRO_SQUARE, PRO_ABS = 0, 1, 2
 EPI_PLAIN, EPI_GATE, EPI_HALF_TANH, EPI_GDN_DIV, EPI_GDN_RSQRT, EPI_GDN_SQRT, EPI_RES_ACT = 0, 1, 2, 3, 4, 5, 6
 MAX_TAPS = 64
-ABI_VERSION = 7   # include/lic.h LIC_ABI_VERSION
+ABI_VERSION = 8   # include/lic.h LIC_ABI_VERSION
 
 EXPORTED_SYMBOLS = (
     "lic_conv2d_fwd", "lic_gdn_prepare", "lic_win_attn_fwd", "lic_layernorm_fwd",
@@ -54,6 +54,8 @@ EXPORTED_SYMBOLS = (
     "lic_resunit_fwd", "lic_patches", "lic_wba_qkv_attn_fwd", "lic_wba16_qkv_attn_fwd", "lic_pack_taps",
     "lic_pack_taps_batch", "lic_pack_block_elems", "lic_rb3_chain_fwd",
     "lic_conv2d_wgrad_partials", "lic_wgrad_reduce_blocks", "lic_wgrad_reduce_batch",
+    "lic_rotary", "lic_quantize_int8", "lic_linear_int8_workspace", "lic_linear_int8",
+    "lic_orthogonalize_workspace", "lic_orthogonalize",
 )
 WGRAD_RED_DESC_WORDS = 16   # include/lic.h LIC_WGRAD_RED_DESC_WORDS
 LIC_EB_PARAMS = 58
@@ -192,6 +194,12 @@ class RansArgs(ctypes.Structure):
     ]
 
 
+class OrthoMat(ctypes.Structure):
+    """lic_ortho_mat (include/lic.h): one matrix of a lic_orthogonalize call."""
+    _fields_ = [("g", _vp), ("rs", ctypes.c_int64), ("cs", ctypes.c_int64), ("out", _vp), ("rows", _i32),
+                ("cols", _i32)]
+
+
 _lib = None
 _load_error = None
 
@@ -271,6 +279,10 @@ def load():
         "lic_resunit_fwd": [V, V],
         "lic_wba_qkv_attn_fwd": [V, V],
         "lic_wba16_qkv_attn_fwd": [V, V],
+        "lic_rotary": [I, V, I, I, I, I, I, I, I, I, I, V, I, V, I, I, V, I, V],
+        "lic_quantize_int8": [I, V, L, I, I, V, I, V, V],
+        "lic_linear_int8": [I, V, L, V, V, I, I, V, I, V, V, I, I, F, V, L, V, L, V, L, V],
+        "lic_orthogonalize": [I, I, V, I, V, F, V, L, V],
         "lic_patches": [I, V, I, I, I, I, I, I, I, I, I, V, V, V, I, I, V],
     }
     for name, argt in sig.items():
@@ -293,6 +305,9 @@ def load():
                        ("lic_wgrad_reduce_blocks", [V])):
         getattr(lib, name).argtypes = argt
         getattr(lib, name).restype = ctypes.c_int32
+    for name, argt in (("lic_linear_int8_workspace", [I, I]), ("lic_orthogonalize_workspace", [I, I, V])):
+        getattr(lib, name).argtypes = argt
+        getattr(lib, name).restype = ctypes.c_int64
     lib.lic_last_error.restype = ctypes.c_char_p
     lib.lic_version.restype = ctypes.c_char_p
     lib.lic_abi_version.restype = ctypes.c_int32
@@ -308,7 +323,8 @@ def load():
     if abi != ABI_VERSION:
         _load_error = f"liblic ABI {abi} at {path}, this host expects {ABI_VERSION}: rebuild liblic.so"
         raise LicError(_load_error)
-    for which, st in enumerate((ConvArgs, AttnArgs, RateArgs, RansArgs, WgradArgs, ResunitArgs, WbaArgs, Wba16Args)):
+    for which, st in enumerate((ConvArgs, AttnArgs, RateArgs, RansArgs, WgradArgs, ResunitArgs, WbaArgs, Wba16Args,
+                                OrthoMat)):
         if lib.lic_args_size(which) != ctypes.sizeof(st):
             _load_error = (f"liblic args struct {st.__name__}: library {lib.lic_args_size(which)} bytes, "
                            f"host {ctypes.sizeof(st)}: rebuild liblic.so")

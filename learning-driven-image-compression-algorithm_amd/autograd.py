@@ -687,6 +687,28 @@ def win_attn(qkv: torch.Tensor, table: torch.Tensor, C: int, heads: int, ws: int
                                          int(mask_kind), bool(scale_after), float(scale)))
 
 
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, plan, heads, inverse):
+        ctx.save_for_backward(positions)
+        ctx.cfg = plan, heads, inverse
+        return Fn.rotary(Act(x.contiguous()), plan, heads, positions, inverse=inverse).t
+
+    @staticmethod
+    def backward(ctx, g):
+        # a rotation's gradient is the rotation back (differentiable again: it is linear)
+        positions, = ctx.saved_tensors
+        plan, heads, inverse = ctx.cfg
+        return _RotaryFn.apply(g, positions, plan, heads, not inverse), None, None, None, None
+
+
+def rotary(x: torch.Tensor, plan: Fn.RotaryPlan, heads: int, positions: Optional[torch.Tensor] = None,
+           inverse: bool = False) -> torch.Tensor:
+    """Rotary positions on the first ``heads`` heads of a [B, H, W, C] tensor, other channels unchanged
+    (functional.rotary, lic_rotary both ways)."""
+    return _RotaryFn.apply(x, positions, plan, int(heads), bool(inverse))
+
+
 # --------------------------------------------------------------------------- rate / reconstruction
 class _RateTrainFn(torch.autograd.Function):
     @staticmethod

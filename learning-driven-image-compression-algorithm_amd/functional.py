@@ -12,6 +12,7 @@ import os
 import threading
 import math
 from dataclasses import dataclass, field
+from fractions import Fraction
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -1061,3 +1062,276 @@ def recon(xtil: Act, wgen: Act, mode: int, post: Optional[torch.Tensor] = None, 
                                _dp(x_rec) if x_rec is not None else None, _dp(parts) if parts is not None else None,
                                ppi, y.ptr if y is not None else None, y.ld if y is not None else 0,
                                y.zpad if y is not None else 0, stream_handle()))
+
+
+# --------------------------------------------------------------------------- rotary positions
+def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The launch goes to the current device's current stream: operands of another device are refused."""
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise ValueError(f"{what}: tensor is not on the GPU (move the module / inputs to 'cuda')")
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != dev:
+            raise ValueError(f"{what}: tensor on {t.device}, the current device is cuda:{dev}")
+
+
+def _overlaps(a: Act, b: Act) -> bool:
+    """Whether two views can share an element (channel windows of one tensor are told apart)."""
+    if not a.t.numel() or a.t.untyped_storage().data_ptr() != b.t.untyped_storage().data_ptr():
+        return False
+    if a.t.data_ptr() == b.t.data_ptr() and a.t.shape == b.t.shape and a.dtype == b.dtype:
+        return a.c0 < b.c0 + b.c and b.c0 < a.c0 + a.c
+    a0, b0 = a.t.data_ptr(), b.t.data_ptr()
+    return a0 < b0 + b.t.numel() * b.t.element_size() and b0 < a0 + a.t.numel() * a.t.element_size()
+
+
+class RotaryPlan:
+    """Which channel pairs of a head turn with which axis, and how fast (lic_rotary).
+
+    ``sections``: the rotated pairs of each axis in order, e.g. (6, 6) for rows and columns, (16, 24, 24) for
+    frames, rows and columns, (32,) for a plain sequence; 2 * sum(sections) <= head_dim, the head's remaining
+    channels pass through.  Pair i of an axis with P pairs turns by position * scale * base ** (-i / P);
+    ``shared_ladder`` counts i and P over all sections together.  ``scale``: one factor, or one per axis (position
+    interpolation).  ``layout``: 'half' pairs channel p with p + sum(sections), 'pairs' 2p with 2p + 1.
+    The angles are kept in 64-bit fixed-point turns, exact for every int32 position."""
+
+    LAYOUTS = {"half": 0, "pairs": 1}
+
+    def __init__(self, head_dim: int, sections: Sequence[int], base: float = 10000.0, scale=1.0, layout: str = "half",
+                 shared_ladder: bool = False, device="cuda"):
+        sections = tuple(int(s) for s in sections)
+        if not 1 <= len(sections) <= 4 or min(sections) < 1:
+            raise ValueError("RotaryPlan: 1 to 4 axes of at least one pair each")
+        if 2 * sum(sections) > head_dim:
+            raise ValueError(f"RotaryPlan: {sum(sections)} pairs do not fit a head of {head_dim} channels")
+        if layout not in self.LAYOUTS:
+            raise ValueError(f"RotaryPlan: layout must be 'half' or 'pairs', got {layout!r}")
+        scales = [float(s) for s in scale] if isinstance(scale, (tuple, list)) else [float(scale)] * len(sections)
+        if len(scales) != len(sections):
+            raise ValueError("RotaryPlan: one scale, or one per axis")
+        if not (base > 0 and math.isfinite(base) and all(math.isfinite(s) for s in scales)):
+            raise ValueError("RotaryPlan: base has to be positive, base and scale finite")
+        self.head_dim, self.sections, self.layout = int(head_dim), sections, layout
+        self.pairs, self.naxes = sum(sections), len(sections)
+        self.freqs: List[float] = []
+        self.axes: List[int] = []
+        for a, count in enumerate(sections):
+            for i in range(count):
+                at = len(self.freqs) / self.pairs if shared_ladder else i / count
+                self.freqs.append(scales[a] * float(base) ** -at)
+                self.axes.append(a)
+        rows = []
+        for f, a in zip(self.freqs, self.axes):
+            turns = round(Fraction(f) / _TWO_PI * 2 ** 64) % 2 ** 64
+            rows.append([turns - 2 ** 64 if turns >= 2 ** 63 else turns, a])
+        self.table = torch.tensor(rows, dtype=torch.int64).to(device)
+
+
+# 2 pi to 40 digits: the turns of a frequency are rounded once
+_TWO_PI = Fraction("6.283185307179586476925286766559005768394")
+
+
+def rotary(x: Act, plan: RotaryPlan, heads: int, positions: Optional[torch.Tensor] = None, out: Optional[Act] = None,
+           inverse: bool = False) -> Act:
+    """Rotate the first ``heads`` heads of plan.head_dim channels of every token of x; the view's other channels are
+    copied.  ``positions``: int32 [naxes, H, W] (every image) or [naxes, B, H, W]; None takes the grid's own: the
+    index y * W + x for one axis, (y, x) for two, (image, y, x) for three.  ``out``: a view of x's size, x itself to
+    rotate in place (then nothing else is touched).  ``inverse`` turns back, which is also the gradient."""
+    if heads < 1 or heads * plan.head_dim > x.c:
+        raise ValueError(f"rotary: {heads} heads of {plan.head_dim} channels do not fit a view of {x.c}")
+    _on_current_device("rotary", x.t, plan.table, positions)
+    per_image = 0
+    if positions is not None:
+        shared = (plan.naxes, x.H, x.W)
+        if positions.dtype != torch.int32 or tuple(positions.shape) not in (shared, (plan.naxes, x.B, x.H, x.W)):
+            raise ValueError(f"rotary: positions must be int32 of shape {shared} or {(plan.naxes, x.B, x.H, x.W)}, got "
+                             f"{positions.dtype} {tuple(positions.shape)}")
+        per_image = 1 if positions.dim() == 4 else 0
+        positions = positions.contiguous()
+    elif plan.naxes > 3:
+        raise ValueError("rotary: four axes need explicit positions")
+    if out is None:
+        out = Act.empty(x.B, x.H, x.W, x.c, x.dtype, x.t.device)
+    else:
+        _on_current_device("rotary", out.t)
+        if (out.B, out.H, out.W, out.c) != (x.B, x.H, x.W, x.c) or out.dtype != x.dtype:
+            raise ValueError("rotary: out has another size or dtype than x")
+        if (out.ptr != x.ptr or out.ld != x.ld) and _overlaps(x, out):
+            raise ValueError("rotary: out overlaps x (only x itself rotates in place)")
+    if x.npix:
+        check(_lib().lic_rotary(dtype_id(x.dtype), x.ptr, x.ld, x.B, x.H, x.W, x.c, heads, plan.head_dim, plan.pairs,
+                                plan.LAYOUTS[plan.layout], _dp(plan.table), plan.naxes,
+                                _dp(positions) if positions is not None else None, per_image, 1 if inverse else 0,
+                                out.ptr, out.ld, stream_handle()))
+    return out
+
+
+# --------------------------------------------------------------------------- products in 8-bit integers
+@dataclass
+class Int8Act:
+    """A map's tokens as 8-bit codes [B, H, W, kpad] (channels beyond c zero) with one fp32 scale each [B, H, W]."""
+    codes: torch.Tensor
+    scale: torch.Tensor
+    c: int
+    dtype: torch.dtype              # of the map that was quantised; linear_int8 answers in it
+
+    @property
+    def shape(self):
+        return self.codes.shape[:3]
+
+
+@dataclass
+class Int8Pack:
+    """A Linear's weights as 8-bit codes [co, kpad] (columns beyond ci zero) with one fp32 scale per output channel."""
+    w: torch.Tensor
+    scale: torch.Tensor
+    bias: Optional[torch.Tensor]    # fp32 [co]
+    ci: int
+
+    @property
+    def co(self):
+        return self.w.shape[0]
+
+
+INT8_MAX_K = 131072
+
+
+def _int8_kpad(k: int) -> int:
+    return -(-k // 64) * 64
+
+
+def _quantize_int8(x_ptr: int, ldx: int, dtype: torch.dtype, m: int, k: int, device):
+    kpad = _int8_kpad(k)
+    codes = torch.empty((m, kpad), dtype=torch.int8, device=device)
+    scale = torch.empty((m,), dtype=torch.float32, device=device)
+    if m:
+        check(_lib().lic_quantize_int8(dtype_id(dtype), x_ptr, ldx, m, k, _dp(codes), kpad, _dp(scale),
+                                       stream_handle()))
+    return codes, scale
+
+
+def quantize_tokens(x: Act) -> Int8Act:
+    """One scale per token, max|x| / 127, and codes rint(127 x / max|x|) (exact, half to even).  A token that holds a
+    NaN or an infinity gets a NaN scale.  For several linear_int8 calls on one map."""
+    _on_current_device("quantize_tokens", x.t)
+    if not 1 <= x.c <= INT8_MAX_K:
+        raise ValueError(f"quantize_tokens: 1 to {INT8_MAX_K} channels, got {x.c}")
+    codes, scale = _quantize_int8(x.ptr, x.ld, x.dtype, x.npix, x.c, x.t.device)
+    return Int8Act(codes.view(x.B, x.H, x.W, -1), scale.view(x.B, x.H, x.W), x.c, x.dtype)
+
+
+def pack_linear_int8(weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> Int8Pack:
+    """nn.Linear weight [co, ci] (fp32, fp16 or bf16) -> 8-bit codes and a scale for each output channel."""
+    if weight.dim() != 2 or not 1 <= weight.shape[1] <= INT8_MAX_K or weight.shape[0] < 1:
+        raise ValueError(f"pack_linear_int8: weight must be [co, ci] with ci up to {INT8_MAX_K}, got "
+                         f"{tuple(weight.shape)}")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError("pack_linear_int8: bias must be [co]")
+    _on_current_device("pack_linear_int8", weight, bias)
+    w = weight.detach().contiguous()
+    codes, scale = _quantize_int8(_dp(w), w.shape[1], w.dtype, w.shape[0], w.shape[1], w.device)
+    return Int8Pack(codes, scale, bias.detach().float().contiguous() if bias is not None else None, w.shape[1])
+
+
+def linear_int8(x, pk: Int8Pack, out: Optional[Act] = None, *, act: int = _ffi.ACT_NONE, slope: float = 0.01,
+                r1: Optional[Act] = None) -> Act:
+    """act(x W^T + bias) + r1 per token of x (an Act, quantised by the call, or an Int8Act) in 8-bit products: integer
+    sums, so equal codes give equal results whatever the batch, the tile or the device.  Forward only."""
+    q = x if isinstance(x, Int8Act) else None
+    B, H, W = q.shape if q is not None else (x.B, x.H, x.W)
+    src = q.codes if q is not None else x.t
+    if x.c != pk.ci:
+        raise ValueError(f"linear_int8: input has {x.c} channels, weights expect {pk.ci}")
+    _on_current_device("linear_int8", src, pk.w, r1.t if r1 is not None else None, out.t if out is not None else None)
+    if act not in (_ffi.ACT_NONE, _ffi.ACT_RELU, _ffi.ACT_LRELU, _ffi.ACT_GELU):
+        raise ValueError("linear_int8: act must be ACT_NONE, ACT_RELU, ACT_LRELU or ACT_GELU")
+    if out is None:
+        out = Act.empty(B, H, W, pk.co, x.dtype, src.device)
+    for v, what in ((out, "out"), (r1, "r1")):
+        if v is not None and ((v.B, v.H, v.W, v.c) != (B, H, W, pk.co) or v.dtype != x.dtype):
+            raise ValueError(f"linear_int8: {what} must be a {x.dtype} view of {(B, H, W, pk.co)}")
+    if q is None and _overlaps(x, out):
+        raise ValueError("linear_int8: out overlaps x")
+    if r1 is not None and (r1.ptr != out.ptr or r1.ld != out.ld) and _overlaps(r1, out):
+        raise ValueError("linear_int8: out overlaps r1 (only r1 itself may be written)")
+    m, kpad = B * H * W, pk.w.shape[1]
+    if m == 0:
+        return out
+    lib = _lib()
+    ws, nbytes = None, 0
+    if q is None:
+        nbytes = int(lib.lic_linear_int8_workspace(m, kpad))
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=src.device)
+    r1p, ldr1 = _ptr(r1)
+    check(lib.lic_linear_int8(dtype_id(x.dtype), None if q is not None else x.ptr, 0 if q is not None else x.ld,
+                              _dp(q.codes) if q is not None else None, _dp(q.scale) if q is not None else None,
+                              m, pk.ci, _dp(pk.w), kpad, _dp(pk.scale), _dp(pk.bias) if pk.bias is not None else None,
+                              pk.co, act, slope, r1p, ldr1, out.ptr, out.ld, _dp(ws) if ws is not None else None,
+                              nbytes, stream_handle()))
+    return out
+
+
+def int8_mode() -> bool:
+    """Whether the calling thread runs Linear layers in 8-bit products."""
+    return getattr(_SPLIT_TLS, "int8", False)
+
+
+class int8_linears:
+    """Context: layers.Linear (the qkv and proj products of the window-attention blocks) runs on linear_int8, weights
+    quantised once per parameter version.  Thread-local, forward only.  Encoder and decoder have to agree on it, as on
+    the precision."""
+
+    def __init__(self, on: bool = True):
+        self.on = bool(on)
+
+    def __enter__(self):
+        self.prev = int8_mode()
+        _SPLIT_TLS.int8 = self.on
+        return self
+
+    def __exit__(self, *exc):
+        _SPLIT_TLS.int8 = self.prev
+        return False
+
+
+# --------------------------------------------------------------------------- orthogonalised updates
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs: Sequence[float] = NEWTON_SCHULZ,
+                  eps: float = 1e-7) -> List[torch.Tensor]:
+    """Newton-Schulz orthogonalisation of every matrix of the list, all in the same few launches: X = G / (|G|_F + eps),
+    then ``steps`` times A = X X^T, X = (a I + b A + c A A) X with coeffs = (a, b, c) (on G^T where G has more rows
+    than columns).  Drives the singular values towards 1: the update direction of the Muon optimiser.
+
+    Matrices: 2-D, of one dtype (fp32, fp16, bf16), any strides.  Returns contiguous matrices of that dtype; everything
+    in between is held in fp32 or in two fp16 parts (22 bits)."""
+    mats = list(mats)
+    if not mats:
+        return []
+    dt = mats[0].dtype
+    for g in mats:
+        if g.dim() != 2 or g.dtype != dt:
+            raise ValueError("orthogonalize: a list of 2-D matrices of one dtype")
+    _on_current_device("orthogonalize", *mats)
+    if len(coeffs) != 3 or not all(math.isfinite(c) for c in coeffs):
+        raise ValueError("orthogonalize: coeffs = (a, b, c), finite")
+    if not 1 <= steps <= 64 or not eps >= 0 or not math.isfinite(eps):
+        raise ValueError("orthogonalize: steps from 1 to 64, eps >= 0")
+    outs = [torch.empty(g.shape, dtype=dt, device=g.device) for g in mats]
+    live = [(g.detach(), o) for g, o in zip(mats, outs) if g.numel()]
+    if not live:
+        return outs
+    desc = (_ffi.OrthoMat * len(live))()
+    for d, (g, o) in zip(desc, live):
+        d.g, d.rs, d.cs, d.out, d.rows, d.cols = g.data_ptr(), g.stride(0), g.stride(1), o.data_ptr(), *g.shape
+    lib = _lib()
+    nbytes = int(lib.lic_orthogonalize_workspace(dtype_id(dt), len(live), desc))
+    if nbytes < 0:
+        raise ValueError("orthogonalize: matrix sizes out of range")
+    ws = torch.empty((nbytes + 256,), dtype=torch.uint8, device=mats[0].device)
+    at = -(-ws.data_ptr() // 256) * 256
+    check(lib.lic_orthogonalize(dtype_id(dt), len(live), desc, steps, (ctypes.c_float * 3)(*coeffs), eps, at, nbytes,
+                                stream_handle()))
+    return outs

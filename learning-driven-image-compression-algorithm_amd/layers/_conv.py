@@ -14,7 +14,7 @@ import torch
 import torch.nn as nn
 
 from .. import functional as Fn
-from .._ffi import ACT_NONE, EPI_PLAIN, PRO_NONE
+from .._ffi import ACT_NONE, ACT_ROUND, EPI_PLAIN, PRO_NONE
 from ..functional import Act
 
 
@@ -98,7 +98,14 @@ class Linear(nn.Linear, _PackCache):
         return self._get_pack(dtype, lambda: Fn.pack_conv2d(self.weight[:, :, None, None], self.bias, 1,
                                                              (0, 0, 0, 0), dtype))
 
+    def packed_int8(self) -> Fn.Int8Pack:
+        return self._get_pack("int8", lambda: Fn.pack_linear_int8(self.weight, self.bias))
+
     def run(self, x: Act, out: Optional[Act] = None, **kw) -> Act:
+        """Inside functional.int8_linears the product runs in 8-bit integers, for the epilogues linear_int8 has
+        (activation and residual); other calls keep the activation dtype's products."""
+        if Fn.int8_mode() and kw.keys() <= {"act", "slope", "r1"} and kw.get("act", ACT_NONE) != ACT_ROUND:
+            return Fn.linear_int8(x, self.packed_int8(), out, **kw)
         return Fn.conv(x, self.packed(x.dtype), out, **kw)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:

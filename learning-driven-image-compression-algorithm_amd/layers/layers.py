@@ -35,11 +35,12 @@ class Win_noShift_Attention(nn.Module):
     The gate and the outer residual are fused into the epilogue of the last conv
     of conv_b; every WBA's shortcut add is fused into its proj launch."""
 
-    def __init__(self, dim, num_heads=8, window_size=8, shift_size=0):
+    def __init__(self, dim, num_heads=8, window_size=8, shift_size=0, rotary=None):
         super().__init__()
         N = dim
         self.conv_a = nn.Sequential(ResidualBlock(N, N), ResidualBlock(N, N), ResidualBlock(N, N))
-        wba = lambda: WinBasedAttention(dim=dim, num_heads=num_heads, window_size=window_size, shift_size=shift_size)
+        wba = lambda: WinBasedAttention(dim=dim, num_heads=num_heads, window_size=window_size, shift_size=shift_size,
+                                        rotary=rotary)
         self.conv_b = nn.Sequential(
             wba(), conv1x1(N, N), wba(), ResidualBlock(N, N), conv3x3(N, N), wba(), ResidualBlock(N, N),
             conv7x7(N, N), wba(), ResidualBlock(N, N))

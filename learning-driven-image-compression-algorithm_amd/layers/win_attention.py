@@ -68,9 +68,16 @@ class WindowAttention(nn.Module):
 
 
 class WinBasedAttention(nn.Module):
+    """``rotary``: a base (e.g. 100.0) turns q and k by their token's row and column before the scores, half of a
+    head's channel pairs each; windows see relative positions only, so the map's coordinates serve shifted windows
+    too.  Parameters and state_dict keys stay those of the block without it (the bias table is still added)."""
+
     def __init__(self, dim=192, num_heads=8, window_size=8, shift_size=0, qkv_bias=True, qk_scale=None, drop=0.,
-                 attn_drop=0., drop_path=0.):
+                 attn_drop=0., drop_path=0., rotary: Optional[float] = None):
         super().__init__()
+        if rotary is not None and (dim // num_heads % 2 or dim // num_heads < 4):
+            raise ValueError(f"rotary needs an even head of at least 4 channels, got {dim // num_heads}")
+        self.rotary = rotary
         self.dim = dim
         self.num_heads = num_heads
         self.window_size = window_size
@@ -79,13 +86,24 @@ class WinBasedAttention(nn.Module):
         self.attn = WindowAttention(dim, window_size=(window_size, window_size), num_heads=num_heads,
                                     qkv_bias=qkv_bias, qk_scale=qk_scale, attn_drop=attn_drop, proj_drop=drop)
 
+    def rotary_plan(self, device) -> Fn.RotaryPlan:
+        """The q / k rotation's plan on a device (kept: it holds only constants)."""
+        plans = self.__dict__.setdefault("_rotary_plans", {})
+        if device not in plans:
+            d = self.dim // self.num_heads
+            plans[device] = Fn.RotaryPlan(d, (d // 4, d // 2 - d // 4), base=self.rotary, device=device)
+        return plans[device]
+
     def run(self, x: Act, out: Optional[Act] = None, **proj_kw) -> Act:
         """out = x + proj(attention(qkv(x))); extra epilogue kwargs go to the proj launch.  Under fp32x6
         at C = 192 / 8 heads / 8x8 windows the qkv Linear and the attention are one launch
         (Fn.wba_qkv_attn: the 3C qkv map never reaches HBM; bit-identical; LIC_FUSED_WBA=0 for the
         three-launch path).  LIC_FUSED_WBA_PROJ=1 also folds the proj + shortcut into that launch
         (bit-identical, but slower today: DESIGN.md section 5)."""
-        if _FUSED and Fn.wba_qkv_attn_ok(x, self.dim, self.num_heads, self.window_size):
+        # rotary positions go between the qkv product and the scores, 8-bit Linears replace the product: both
+        # take the three-launch path
+        plain = self.rotary is None and not Fn.int8_mode()
+        if plain and _FUSED and Fn.wba_qkv_attn_ok(x, self.dim, self.num_heads, self.window_size):
             # the fused proj stores 16 B per lane: only into a fresh buffer or a 16-B aligned view
             # with 4-element rows, never onto x (the shortcut) -- else the proj runs as its own launch
             fuse_proj = _FUSED_PROJ and not proj_kw and (
@@ -96,13 +114,16 @@ class WinBasedAttention(nn.Module):
                                 out=out if fuse_proj else None,
                                 proj_pk=self.attn.proj.packed(x.dtype) if fuse_proj else None)
             return a if fuse_proj else self.attn.proj.run(a, out, r1=x, **proj_kw)
-        if _FUSED16 and Fn.wba16_qkv_attn_ok(x, self.dim, self.num_heads, self.window_size):
+        if plain and _FUSED16 and Fn.wba16_qkv_attn_ok(x, self.dim, self.num_heads, self.window_size):
             # 16-bit: qkv + attention in one launch (csrc/wba16.hip); LIC_FUSED_WBA16=0 for two launches
             a = Fn.wba16_qkv_attn(x, self.attn.qkv.packed(x.dtype), self.num_heads, self.window_size,
                                   self.shift_size, self.attn.relative_position_bias_table, self.num_heads, 1,
                                   1 if self.shift_size > 0 else 0, float(self.attn.scale))
             return self.attn.proj.run(a, out, r1=x, **proj_kw)
         qkv = self.attn.qkv.run(x)
+        if self.rotary is not None:
+            qk = qkv.ch(0, 2 * self.dim)
+            Fn.rotary(qk, self.rotary_plan(x.t.device), 2 * self.num_heads, out=qk)
         a = Fn.win_attn(qkv, self.dim, self.num_heads, self.window_size, self.shift_size,
                         self.attn.relative_position_bias_table, self.num_heads, 1,
                         1 if self.shift_size > 0 else 0, False, float(self.attn.scale))

@@ -1,0 +1,91 @@
+"""Optimisers whose updates run on liblic."""
+from __future__ import annotations
+
+import math
+from typing import Iterable, List, Tuple
+
+import torch
+import torch.nn as nn
+
+from . import functional as Fn
+
+__all__ = ["Muon", "split_muon_params"]
+
+
+def split_muon_params(module: nn.Module, params: Iterable[torch.Tensor]) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:
+    """(matrices, others) of ``params``: the weights of module's dense convolutions, transposed convolutions and Linears
+    with at least 8 rows and columns, and everything else (biases, GDN parameters, bias tables, depthwise filters)."""
+    dense = set()
+    for m in module.modules():
+        if isinstance(m, (nn.Conv2d, nn.ConvTranspose2d, nn.Linear)) and getattr(m, "groups", 1) == 1:
+            w = m.weight
+            if min(w.shape[0], w[0].numel()) >= 8:
+                dense.add(id(w))
+    params = list(params)
+    return [p for p in params if id(p) in dense], [p for p in params if id(p) not in dense]
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update is orthogonalised (functional.orthogonalize): every weight moves by
+    lr * scale * NewtonSchulz(u), u the (Nesterov) momentum of its gradient as a matrix [shape[0], rest].
+
+    ``adjust``: 'rms' scales by 0.2 sqrt(max(rows, cols)), an update of root mean square about 0.2 whatever the shape
+    (Adam's learning rates carry over); 'shape' by sqrt(max(1, rows / cols)).  ``weight_decay`` is decoupled.  The
+    momentum is fp32, all matrices of a dtype are orthogonalised in the same few launches, and the result is the same
+    bits on every rank that holds the same gradients.  ``lr`` may be a device scalar: the step then captures into a
+    hipGraph (after one eager step, which creates the momentum)."""
+
+    def __init__(self, params, lr=1e-3, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+                 steps: int = 5, adjust: str = "rms", eps: float = 1e-7):
+        if not isinstance(lr, torch.Tensor) and not lr >= 0:
+            raise ValueError(f"Muon: lr must be >= 0, got {lr}")
+        if not 0 <= momentum < 1 or not weight_decay >= 0:
+            raise ValueError("Muon: momentum in [0, 1), weight_decay >= 0")
+        if adjust not in ("rms", "shape"):
+            raise ValueError(f"Muon: adjust must be 'rms' or 'shape', got {adjust!r}")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      steps=steps, adjust=adjust, eps=eps))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() < 2:
+                    raise ValueError("Muon: matrices and filters only (give vectors to another optimiser)")
+
+    @staticmethod
+    def _scale(adjust: str, rows: int, cols: int) -> float:
+        return 0.2 * math.sqrt(max(rows, cols)) if adjust == "rms" else math.sqrt(max(1.0, rows / cols))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            lr, mu, wd = group["lr"], group["momentum"], group["weight_decay"]
+            bufs = []
+            for p in params:
+                st = self.state[p]
+                if "momentum" not in st:
+                    st["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                bufs.append(st["momentum"])
+            grads = [p.grad.float() for p in params]
+            # m <- mu m + (1 - mu) g;  u = mu m + (1 - mu) g (Nesterov) or m
+            torch._foreach_lerp_(bufs, grads, 1.0 - mu)
+            ups = torch._foreach_lerp(bufs, grads, 1.0 - mu) if group["nesterov"] else bufs
+            mats = [u.reshape(u.shape[0], -1) for u in ups]
+            orth = Fn.orthogonalize(mats, steps=group["steps"], eps=group["eps"])
+            orth = [o.view(p.shape).to(p.dtype) for o, p in zip(orth, params)]
+            torch._foreach_mul_(orth, [self._scale(group["adjust"], *m.shape) for m in mats])
+            if isinstance(lr, torch.Tensor):
+                torch._foreach_mul_(orth, lr)
+                if wd:
+                    torch._foreach_mul_(params, 1.0 - lr * wd)
+                torch._foreach_sub_(params, orth)
+            else:
+                if wd:
+                    torch._foreach_mul_(params, 1.0 - lr * wd)
+                torch._foreach_sub_(params, orth, alpha=lr)
+        return loss

@@ -116,6 +116,8 @@ def wba(m, x):
     """WinBasedAttention (layers/win_attention.py:154-209): x + proj(attn(qkv(x)))."""
     at = m.attn
     qkv = linear(at.qkv, x)
+    if m.rotary is not None:
+        qkv = AG.rotary(qkv, m.rotary_plan(qkv.device), 2 * m.num_heads)
     a = AG.win_attn(qkv, at.relative_position_bias_table, m.dim, m.num_heads, m.window_size, m.shift_size,
                     tab_sr=m.num_heads, tab_sh=1, mask_kind=1 if m.shift_size > 0 else 0, scale_after=False,
                     scale=float(at.scale))

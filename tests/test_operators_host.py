@@ -1,0 +1,227 @@
+"""Rotary plans and the refusals of the rotary, 8-bit and orthogonalisation operators (no GPU: every call here is
+refused before anything is launched, or never reaches the device)."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import lic_amd
+import lic_amd.functional as Fn
+from lic_amd import _ffi
+from lic_amd.functional import Act
+
+
+def _plan(*a, **k):
+    return Fn.RotaryPlan(*a, device="cpu", **k)
+
+
+def test_rotary_plan_frequencies():
+    p = _plan(32, (4, 6), base=100.0, scale=(1.0, 0.5))
+    assert p.pairs == 10 and p.naxes == 2 and p.axes == [0] * 4 + [1] * 6
+    want = [100.0 ** (-i / 4) for i in range(4)] + [0.5 * 100.0 ** (-i / 6) for i in range(6)]
+    assert p.freqs == pytest.approx(want, rel=1e-15)
+    shared = _plan(32, (4, 6), base=100.0, shared_ladder=True)
+    assert shared.freqs == pytest.approx([100.0 ** (-i / 10) for i in range(10)], rel=1e-15)
+
+
+@pytest.mark.parametrize("pos", [0, 1, -1, 12345, 2 ** 31 - 1, -2 ** 31])
+def test_rotary_table_angles(pos):
+    """The fixed-point turns times any int32 position, modulo 2^64, is the angle modulo one turn: off by at most
+    |pos| / 2 steps of 2^-64 turns (the table's rounding: |pos| pi 2^-64 rad), the 64-bit reference's own rounding of
+    pos * freq (2^-53 relative) and its 2 pi (2.5e-16 off, once a turn: under pos * freq * 2^-54)."""
+    p = _plan(64, (16,), base=10000.0)
+    for turns, freq in zip(p.table[:, 0].tolist(), p.freqs):
+        got = (turns * pos) % 2 ** 64 / 2 ** 64 * 2 * math.pi
+        want = pos * freq
+        tol = abs(pos) * math.pi * 2 ** -64 + abs(pos) * freq * 2 ** -51 + 1e-12
+        assert abs(math.remainder(got - want, 2 * math.pi)) <= tol
+
+
+@pytest.mark.parametrize("args,kw", [((16, ()), {}), ((16, (4, 5)), {}), ((16, (4, 0)), {}), ((64, (1,) * 5), {}),
+                                     ((16, (4,)), {"layout": "thirds"}), ((16, (4,)), {"base": 0.0}),
+                                     ((16, (4, 4)), {"scale": (1.0,)}), ((16, (4,)), {"scale": float("inf")})])
+def test_rotary_plan_refusals(args, kw):
+    with pytest.raises(ValueError, match="RotaryPlan"):
+        _plan(*args, **kw)
+
+
+def test_host_tensors_are_refused():
+    x = Act(torch.zeros(1, 2, 2, 32))
+    with pytest.raises(ValueError, match="not on the GPU"):
+        Fn.rotary(x, _plan(16, (4,)), 2)
+    with pytest.raises(ValueError, match="not on the GPU"):
+        Fn.quantize_tokens(x)
+    with pytest.raises(ValueError, match="not on the GPU"):
+        Fn.pack_linear_int8(torch.zeros(4, 32))
+    with pytest.raises(ValueError, match="not on the GPU"):
+        Fn.linear_int8(x, Fn.Int8Pack(torch.zeros(4, 64, dtype=torch.int8), torch.ones(4), None, 32))
+    with pytest.raises(ValueError, match="not on the GPU"):
+        Fn.orthogonalize([torch.zeros(4, 4)])
+
+
+def test_size_refusals():
+    x = Act(torch.zeros(1, 2, 2, 32))
+    with pytest.raises(ValueError, match="do not fit"):
+        Fn.rotary(x, _plan(16, (4,)), 3)
+    with pytest.raises(ValueError, match="do not fit"):
+        Fn.rotary(x, _plan(16, (4,)), 0)
+    with pytest.raises(ValueError, match="channels"):
+        Fn.linear_int8(x, Fn.Int8Pack(torch.zeros(4, 64, dtype=torch.int8), torch.ones(4), None, 31))
+    with pytest.raises(ValueError, match="weight must be"):
+        Fn.pack_linear_int8(torch.zeros(4, 4, 1))
+    with pytest.raises(ValueError, match="bias"):
+        Fn.pack_linear_int8(torch.zeros(4, 4), torch.zeros(5))
+    with pytest.raises(ValueError, match="one dtype"):
+        Fn.orthogonalize([torch.zeros(4, 4), torch.zeros(4, 4, dtype=torch.float16)])
+    with pytest.raises(ValueError, match="one dtype"):
+        Fn.orthogonalize([torch.zeros(4)])
+    assert Fn.orthogonalize([]) == []
+
+
+def test_overlap_rule():
+    t = torch.zeros(1, 2, 2, 32)
+    a = Act(t, 0, 16)
+    assert Fn._overlaps(a, Act(t, 8, 16)) and Fn._overlaps(a, a)
+    assert not Fn._overlaps(a, Act(t, 16, 16)) and not Fn._overlaps(a, Act(torch.zeros(1, 2, 2, 32)))
+    assert not Fn._overlaps(Act(t[:, :1].clone()), Act(t)) and Fn._overlaps(Act(t[:, 1:]), Act(t))
+    assert not Fn._overlaps(Act(t[:, :1]), Act(t[:, 1:])) and not Fn._overlaps(Act(t[:0]), Act(t[:0]))
+    assert Fn._overlaps(Act(t.view(1, 1, 4, 32), 0, 16), Act(t, 16, 16))   # other shapes: refused on byte ranges
+
+
+def _refused(status, text):
+    assert status != 0 and text in _ffi._lib.lic_last_error().decode(), _ffi._lib.lic_last_error()
+
+
+def test_c_entry_refusals():
+    """Arguments the C ABI refuses; the fake pointers are never read."""
+    lib = lic_amd.load_library()
+    f = 4096   # a non-null, aligned address that nothing dereferences
+
+    def rot(dtype=0, x=f, ldx=64, n=1, h=2, w=2, c=64, heads=2, dim=32, pairs=8, layout=0, table=f, naxes=2, pos=None,
+            y=f, ldy=64):
+        return lib.lic_rotary(dtype, x, ldx, n, h, w, c, heads, dim, pairs, layout, table, naxes, pos, 0, 0, y, ldy,
+                              None)
+    _refused(rot(dtype=7), "dtype")
+    _refused(rot(heads=3), "fit the view")
+    _refused(rot(heads=2 ** 30, dim=2 ** 30), "fit the view")
+    _refused(rot(pairs=17), "fit the view")
+    _refused(rot(pairs=0), "fit the view")
+    _refused(rot(ldx=63), "fit the view")
+    _refused(rot(layout=2), "layout")
+    _refused(rot(naxes=0), "naxes")
+    _refused(rot(naxes=4), "naxes")
+    _refused(rot(naxes=5, pos=f), "naxes")
+    _refused(rot(n=-1), "negative")
+    _refused(rot(table=None), "null")
+    _refused(rot(y=f, ldy=80), "in place")
+    assert rot(n=0) == 0
+
+    def quant(dtype=0, x=f, ldx=100, m=4, k=100, codes=f, kpad=128, scale=f):
+        return lib.lic_quantize_int8(dtype, x, ldx, m, k, codes, kpad, scale, None)
+    _refused(quant(dtype=3), "dtype")
+    _refused(quant(kpad=96), "out of range")
+    _refused(quant(kpad=100), "out of range")
+    _refused(quant(k=0), "out of range")
+    _refused(quant(k=200000, kpad=200000), "out of range")
+    _refused(quant(m=-1), "out of range")
+    _refused(quant(ldx=99), "stride")
+    _refused(quant(codes=f + 8), "aligned")
+    assert quant(m=0) == 0
+
+    def lin(dtype=0, x=f, ldx=100, xc=None, xs=None, m=4, k=100, w=f, kpad=128, ws=f, n=8, act=0, r1=None, ldr1=0, y=f,
+            ldy=8, work=f, nbytes=1 << 20):
+        return lib.lic_linear_int8(dtype, x, ldx, xc, xs, m, k, w, kpad, ws, None, n, act, 0.0, r1, ldr1, y, ldy, work,
+                                   nbytes, None)
+    _refused(lin(dtype=-1), "dtype")
+    _refused(lin(n=0), "n out of range")
+    _refused(lin(act=4), "act")
+    _refused(lin(ldy=7), "stride below n")
+    _refused(lin(r1=f, ldr1=7), "stride below n")
+    _refused(lin(x=None), "x or xcodes")
+    _refused(lin(xc=f, xs=f), "x or xcodes")
+    _refused(lin(x=None, xc=f), "x or xcodes")
+    _refused(lin(w=f + 4), "aligned")
+    _refused(lin(ldx=99), "stride below k")
+    _refused(lin(work=None), "workspace")
+    _refused(lin(nbytes=16), "workspace")
+    assert lin(m=0) == 0
+    assert lib.lic_linear_int8_workspace(4, 128) > 4 * 128 and lib.lic_linear_int8_workspace(-1, 128) == -1
+
+    def ortho(rows=8, cols=8, g=f, out=f, steps=5, eps=1e-7, dtype=0, count=1, ws=f, nbytes=1 << 30, coeffs=True):
+        m = (_ffi.OrthoMat * 1)()
+        m[0].g, m[0].rs, m[0].cs, m[0].out, m[0].rows, m[0].cols = g, max(cols, 1), 1, out, rows, cols
+        co = (ctypes.c_float * 3)(*Fn.NEWTON_SCHULZ) if coeffs else None
+        return lib.lic_orthogonalize(dtype, count, m, steps, co, eps, ws, nbytes, None)
+    _refused(ortho(rows=0), "out of range")
+    _refused(ortho(rows=65537), "out of range")
+    _refused(ortho(g=None), "null")
+    _refused(ortho(out=None), "null")
+    _refused(ortho(steps=0), "steps")
+    _refused(ortho(eps=-1.0), "eps")
+    _refused(ortho(eps=float("nan")), "eps")
+    _refused(ortho(dtype=9), "dtype")
+    _refused(ortho(count=-1), "null")
+    _refused(ortho(coeffs=False), "null")
+    _refused(ortho(ws=None), "workspace")
+    _refused(ortho(ws=f + 8), "workspace")
+    _refused(ortho(nbytes=64), "workspace")
+    assert ortho(count=0) == 0
+
+
+def test_ortho_struct_matches_c_compiler(tmp_path):
+    import shutil
+    import subprocess
+    if shutil.which("gcc") is None:
+        pytest.skip("gcc not available")
+    from tests.test_capi import ROOT
+    py = _ffi.OrthoMat
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "lic.h"\nint main(void) {\n'
+                   'printf("%zu", sizeof(lic_ortho_mat));\n' +
+                   "".join(f'printf(" %zu", offsetof(lic_ortho_mat, {n[0]}));\n' for n in py._fields_) + "return 0; }")
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [ctypes.sizeof(py)] + [getattr(py, n[0]).offset for n in py._fields_]
+    assert lic_amd.load_library().lic_args_size(8) == ctypes.sizeof(py)
+
+
+def test_muon_refusals_and_split():
+    from lic_amd.layers import Conv2d, ConvTranspose2d, Linear
+    from lic_amd.optim import Muon, split_muon_params
+    net = torch.nn.Sequential(Conv2d(16, 32, 3), Conv2d(16, 16, 3, groups=16), ConvTranspose2d(32, 16, 5), Linear(16, 4),
+                              torch.nn.LayerNorm(16))
+    mats, others = split_muon_params(net, net.parameters())
+    assert [tuple(p.shape) for p in mats] == [(32, 16, 3, 3), (32, 16, 5, 5)]
+    assert len(mats) + len(others) == len(list(net.parameters()))
+    with pytest.raises(ValueError, match="matrices"):
+        Muon([torch.nn.Parameter(torch.zeros(4))])
+    with pytest.raises(ValueError, match="adjust"):
+        Muon(mats, adjust="none")
+    with pytest.raises(ValueError, match="momentum"):
+        Muon(mats, momentum=1.0)
+    with pytest.raises(ValueError, match="lr"):
+        Muon(mats, lr=-1.0)
+
+
+def test_int8_context_is_nested_and_thread_local():
+    import threading
+    assert not Fn.int8_mode()
+    seen = []
+    with Fn.int8_linears():
+        t = threading.Thread(target=lambda: seen.append(Fn.int8_mode()))
+        t.start()
+        t.join()
+        with Fn.int8_linears(False):
+            assert not Fn.int8_mode()
+        assert Fn.int8_mode()
+    assert not Fn.int8_mode() and seen == [False]
+
+
+def test_rotary_block_refusal():
+    from lic_amd.layers import WinBasedAttention
+    with pytest.raises(ValueError, match="even head"):
+        WinBasedAttention(24, 8, 8, rotary=100.0)
+    plain, turned = WinBasedAttention(32, 4, 8), WinBasedAttention(32, 4, 8, rotary=100.0)
+    assert plain.state_dict().keys() == turned.state_dict().keys()

@@ -71,6 +71,9 @@ def main():
     ap.add_argument("--post_processing", action="store_true", help="Using Post Processing (not trainable yet)")
     ap.add_argument("--lambda", type=float, default=0.0025, dest="lmbda")
     ap.add_argument("--lr", type=float, default=1e-4)
+    ap.add_argument("--optimizer", default="adam", choices=["adam", "muon"],
+                    help="muon: the dense convolution and Linear weights by lic_amd.optim.Muon (orthogonalised "
+                         "momentum), everything else by Adam, both at --lr")
     ap.add_argument("--batch_size", type=float, default=8, help="images per GPU")
     ap.add_argument("--precision", default="bf16", choices=["bf16", "fp16", "fp32"],
                     help="activation dtype (fp32 master weights, fp32 accumulation); bf16 = BASELINE config 5")
@@ -138,9 +141,18 @@ def main():
     # capturable Adam keeps lr and the step count on the device (graph replays update them); fused:
     # one multi-tensor kernel per step -- the foreach path with a device lr falls back to one
     # broadcast division per parameter (~1000 launches per step, rocprofv3 trace r04v)
-    opt = torch.optim.Adam(params, lr=torch.tensor(args.lr, device=dev) if args.graph else args.lr,
-                           capturable=args.graph, fused=os.environ.get("LIC_FUSED_ADAM", "1") != "0")
-    sch = torch.optim.lr_scheduler.MultiStepLR(opt, [1500, 2500, 3500, 4000], 0.5)
+    def learning_rate():
+        return torch.tensor(args.lr, device=dev) if args.graph else args.lr
+
+    matrices, others = [], params
+    if args.optimizer == "muon":
+        from lic_amd.optim import Muon, split_muon_params
+        matrices, others = split_muon_params(net, params)
+    opts = [torch.optim.Adam(others, lr=learning_rate(), capturable=args.graph,
+                             fused=os.environ.get("LIC_FUSED_ADAM", "1") != "0")]
+    if matrices:
+        opts.append(Muon(matrices, lr=learning_rate()))
+    schs = [torch.optim.lr_scheduler.MultiStepLR(o, [1500, 2500, 3500, 4000], 0.5) for o in opts]
     sync = D.GradAllReduce(params, world)
     # one GPU: the backward's split-K wgrad reduces as one launch after it (autograd.WgradDefer; at
     # world > 1 the eager GradAllReduce hooks read .grad during the backward).  LIC_WGRAD_DEFER=0: off
@@ -157,13 +169,21 @@ def main():
 
     grad_params = None
 
+    def zero_grad():
+        for o in opts:
+            o.zero_grad(set_to_none=True)
+
+    def opt_step():
+        for o in opts:
+            o.step()
+
     def step_body(x, seed_dev=None):
         bpp, mse = net(x, "train", seed_dev=seed_dev)
         loss = args.lmbda * 255 ** 2 * mse + bpp                       # :180
         backward(loss)
         sync.finish()                                                  # RCCL all-reduce, captured too
         torch.nn.utils.clip_grad_norm_(grad_params, 1.0)               # :198
-        opt.step()
+        opt_step()
         return loss.detach(), bpp.detach(), mse.detach()
 
     if args.graph:
@@ -178,17 +198,17 @@ def main():
         nwarm = max(2 if plan is not None else 1, args.warmup)
         with torch.cuda.stream(side):
             for k in range(nwarm):
-                opt.zero_grad(set_to_none=True)
+                zero_grad()
                 with plan.record() if (plan is not None and k == nwarm - 1) else contextlib.nullcontext():
                     bpp, mse = net(static_x, "train", seed_dev=seed_t)
                     backward(args.lmbda * 255 ** 2 * mse + bpp)
                 sync.finish()              # first collectives eagerly: communicator set up before capture
                 grad_params = [p for p in clip_params if p.grad is not None]
                 torch.nn.utils.clip_grad_norm_(grad_params, 1.0)
-                opt.step()
+                opt_step()
                 seed_t.add_(1)
         torch.cuda.current_stream().wait_stream(side)
-        opt.zero_grad(set_to_none=True)
+        zero_grad()
         if plan is not None:
             plan.finalize()
         torch.cuda.synchronize(dev)   # the warm-up's collectives complete before the capture starts
@@ -215,14 +235,16 @@ def main():
 
     def eager_step():
         x = batches()
-        opt.zero_grad(set_to_none=True)
+        zero_grad()
         bpp, mse = net(x, "train")
         loss = args.lmbda * 255 ** 2 * mse + bpp                       # :180
         backward(scaler.scale(loss))
         sync.finish()
-        scaler.unscale_(opt)
+        for o in opts:
+            scaler.unscale_(o)
         torch.nn.utils.clip_grad_norm_([p for p in clip_params if p.grad is not None], 1.0)   # :198
-        scaler.step(opt)
+        for o in opts:
+            scaler.step(o)
         scaler.update()
         return loss.detach(), bpp.detach(), mse.detach()
 
@@ -249,7 +271,8 @@ def main():
                 "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
                 "dtype": {"fp16": "f16", "bf16": "bf16"}.get(args.precision, "f32"),
                 "data": "synthetic (seeded smooth images, random crops in HBM; no DIV2K)",
-                "config": {"workload": f"{args.arch} Net.forward(x,'train') + backward + grad all-reduce + clip + Adam",
+                "config": {"workload": f"{args.arch} Net.forward(x,'train') + backward + grad all-reduce + clip + "
+                                       + ("Adam" if args.optimizer == "adam" else "Muon and Adam"),
                            "global_batch": world * B, "crop": args.crop, "lambda": args.lmbda,
                            "parallelism": f"data-parallel x{world} (bucketed RCCL all-reduce)",
                            "execution": "hipGraph replay of the whole step" if args.graph else "eager"},
@@ -269,7 +292,8 @@ def main():
                     raise Exception("NaN in loss")                      # :189-190
                 sums = [s + v for s, v in zip(sums, vals)]
                 acc = None
-        sch.step()
+        for sch in schs:
+            sch.step()
         cnt = args.steps_per_epoch
         if rank == 0:
             msg = "[Epoch %04d TRAIN] Loss: %.4f bpp: %.4f mse: %.4f  " % (epoch, sums[0] / cnt, sums[1] / cnt,
