@@ -699,7 +699,9 @@ class _RotaryFn(torch.autograd.Function):
         # a rotation's gradient is the rotation back (differentiable again: it is linear)
         positions, = ctx.saved_tensors
         plan, heads, inverse = ctx.cfg
-        return _RotaryFn.apply(g, positions, plan, heads, not inverse), None, None, None, None
+        if torch.is_grad_enabled():
+            return _RotaryFn.apply(g, positions, plan, heads, not inverse), None, None, None, None
+        return Fn.rotary(Act(g.contiguous()), plan, heads, positions, inverse=not inverse).t, None, None, None, None
 
 
 def rotary(x: torch.Tensor, plan: Fn.RotaryPlan, heads: int, positions: Optional[torch.Tensor] = None,
