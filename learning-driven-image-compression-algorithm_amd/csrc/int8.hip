@@ -3,51 +3,106 @@
 
 namespace lic {
 
-// code = rint(127 x / amax), half to even, exactly.  x and amax are first scaled by one power of two (amax to
-// [1, 2)), so nothing overflows; the fp32 quotient is exact enough except next to a border k + 1/2, which is
-// decided in 64 bits, where 254 x and (2k + 1) amax are exact.
-__device__ __forceinline__ int quant_code(float x, float amax) {
-  const float t = x * 127.f / amax;
-  float q = rintf(t);
-  const float d = t - q;
-  if (fabsf(fabsf(d) - 0.5f) < 1e-4f) {
-    const double lo = floor((double)t);   // t is within 1e-4 of lo + 1/2
-    const double diff = 254.0 * (double)x - (2.0 * lo + 1.0) * (double)amax;
-    q = (float)(diff > 0 ? lo + 1 : diff < 0 ? lo : 2.0 * rint(lo * 0.5 + 0.25));
-  }
-  return (int)q;
-}
+template <typename T, int V> using QuantVec = T __attribute__((ext_vector_type(V)));
 
-// Largest magnitude of a row; NaN if the row holds a NaN or an infinity.
-__device__ __forceinline__ float quant_absmax(float m, float v) {
-  const float a = fabsf(v);
-  return a <= m ? m : (a < INFINITY ? (m == m ? a : m) : NAN);
-}
-
-// The largest magnitude of two running ones (NaN wins).
-__device__ __forceinline__ float quant_max2(float a, float b) { return b != b ? b : (b > a ? b : a); }
-
-// A row's power-of-two scaling and the scaled maximum; `live` is false for zero rows and NaN (codes 0).
+// A row's codes: rint(127 x / top), half to even, exactly.  The fp32 product t = x * (127 / top) is within |t| 2^-22.4 of the
+// quotient.  16-bit x: a quotient that is no border k + 1/2 is at least |t| 2^-19 away from one (254 X - (2k + 1) T is a whole
+// number in units of x's last place, X < 2^11), so only exact borders can be missed, and a t that near to a border is one.
+// fp32 x: next to a border 254 x is compared with (2k + 1) top in two floats each, exactly.  Rows outside 2^-100 .. 2^100
+// are scaled by a power of two, so nothing overflows or loses bits.
 struct QuantRow {
-  float amax;
-  int shift;
-  bool live;
+  float top, scale, inv;   // scaled maximum, the scaling, 127 / top; inv 0: a zero row or one with a NaN or an infinity
 };
 __device__ __forceinline__ QuantRow quant_row(float top) {
-  QuantRow q{1.f, 0, top > 0.f};
-  if (q.live) {
-    int e;
-    (void)frexpf(top, &e);
-    q.shift = 1 - e;
-    q.amax = ldexpf(top, q.shift);
-  }
+  const float scale = top < 7.9e-31f ? 18446744073709551616.f : top > 1.2e30f ? 5.421010862427522e-20f : 1.f;
+  QuantRow q{top * scale, scale, 0.f};
+  if (top > 0.f) q.inv = 127.f / q.top;
   return q;
 }
-__device__ __forceinline__ int quant_code(float x, const QuantRow& q) {
-  return q.live ? quant_code(ldexpf(x, q.shift), q.amax) : 0;
+constexpr float QUANT_ROUND = 12582912.f;   // 1.5 * 2^23: adding it rounds, and leaves the integer in the low bits
+// N codes packed four to a word (the last word's missing ones 0)
+template <typename T, int N>
+__device__ __forceinline__ void quant_codes(const float* x, const QuantRow& q, uint32_t* out) {
+#pragma clang fp contract(off)   // every product below is a rounded one
+  float t[N], r[N];
+  if (q.scale == 1.f) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) t[e] = x[e] * q.inv;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) t[e] = x[e] * q.scale * q.inv;
+  }
+  float far = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    r[e] = t[e] + QUANT_ROUND;
+    far = fmaxf(far, fabsf(t[e] - (r[e] - QUANT_ROUND)));
+  }
+  if (far > 0.5f - 4e-5f) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float n = r[e] - QUANT_ROUND, d = t[e] - n;
+      if (fabsf(d) > 0.5f - fabsf(t[e]) * 3e-7f) {
+        const float even = 2.f * rintf(0.5f * t[e]);
+        if constexpr (sizeof(T) == 2) {
+          r[e] = even + QUANT_ROUND;
+        } else {
+          const float b2 = 2.f * n + (d > 0.f ? 1.f : -1.f), xs = x[e] * q.scale;   // the border, doubled
+          const float h0 = 254.f * xs, h1 = b2 * q.top;
+          const float l0 = fmaf(254.f, xs, -h0), l1 = fmaf(b2, q.top, -h1);
+          const float diff = (h0 - h1) + (l0 - l1);
+          r[e] = (diff > 0.f ? 0.5f * (b2 + 1.f) : diff < 0.f ? 0.5f * (b2 - 1.f) : even) + QUANT_ROUND;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < (N + 3) / 4; ++w) {
+    uint32_t b[4] = {};
+#pragma unroll
+    for (int e = 0; e < 4 && 4 * w + e < N; ++e) b[e] = __float_as_uint(r[4 * w + e]);
+    // the low bytes of four words
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+    out[w] = lo | hi;
+  }
 }
 
-template <typename T, int V> using QuantVec = T __attribute__((ext_vector_type(V)));
+// Magnitudes are compared as bit patterns, where infinities and NaN are the largest (16-bit types two at a time).
+template <typename T> struct QuantMax {
+  typedef unsigned short Two __attribute__((ext_vector_type(2)));
+  Two m{};
+  template <typename Vec> __device__ __forceinline__ void add(const Vec& v) {
+    constexpr int V = sizeof(Vec) / 2;
+    if constexpr (V == 1) {
+      const unsigned short b = __builtin_bit_cast(unsigned short, v[0]) & 0x7fff;
+      m[0] = b > m[0] ? b : m[0];
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const T two[2] = {v[e], v[e + 1]};
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(Two, __builtin_bit_cast(uint32_t, two) & 0x7fff7fffu));
+      }
+    }
+  }
+  __device__ __forceinline__ uint32_t bits() const { return m[0] > m[1] ? m[0] : m[1]; }
+  // the magnitude; NaN for an infinity or a NaN (then also the row's scale, and its results)
+  static __device__ __forceinline__ float value(uint32_t b) {
+    const float f = to_f(__builtin_bit_cast(T, (unsigned short)b));
+    return f < INFINITY ? f : NAN;
+  }
+};
+template <> struct QuantMax<float> {
+  uint32_t m = 0;
+  template <typename Vec> __device__ __forceinline__ void add(const Vec& v) {
+#pragma unroll
+    for (int e = 0; e < (int)(sizeof(Vec) / 4); ++e) {
+      const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
+      m = b > m ? b : m;
+    }
+  }
+  __device__ __forceinline__ uint32_t bits() const { return m; }
+  static __device__ __forceinline__ float value(uint32_t b) { return b < 0x7f800000u ? __uint_as_float(b) : NAN; }
+};
 
 // G lanes a row, V elements a load; a lane keeps its part of the row in registers (NV vectors of it; longer rows are read
 // a second time).  Bound by the bytes of x and codes.
@@ -62,35 +117,43 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(const T* __restrict_
   if (row >= m) return;
   const T* xr = x + row * ldx;
   Vec v[NV];
-  float top = 0.f;
+  QuantMax<T> most;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    v[i] = Vec{};
     if ((lane + i * G) * V < k) v[i] = *(const Vec*)(xr + (lane + i * G) * V);
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if ((lane + i * G) * V < k)
-#pragma unroll
-      for (int e = 0; e < V; ++e) top = quant_absmax(top, to_f(v[i][e]));
-  for (int j = (lane + NV * G) * V; j < k; j += G * V) {
-    const Vec u = *(const Vec*)(xr + j);
-#pragma unroll
-    for (int e = 0; e < V; ++e) top = quant_absmax(top, to_f(u[e]));
   }
 #pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) top = quant_max2(top, __shfl_xor(top, o));
+  for (int i = 0; i < NV; ++i) most.add(v[i]);
+  for (int j = (lane + NV * G) * V; j < k; j += G * V) most.add(*(const Vec*)(xr + j));
+  uint32_t bits = most.bits();
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) {
+    const uint32_t other = __shfl_xor(bits, o);
+    bits = other > bits ? other : bits;
+  }
+  const float top = QuantMax<T>::value(bits);
   if (lane == 0) scale[row] = top / 127.f;
   const QuantRow q = quant_row(top);
   typedef QuantVec<int8_t, V> Codes;
   Codes* cr = (Codes*)(codes + row * kpad);
   auto put = [&](const Vec& u, int j) {
-    Codes c;
+    float f[V];
+    uint32_t w[(V + 3) / 4];
 #pragma unroll
-    for (int e = 0; e < V; ++e) c[e] = j < k ? (int8_t)quant_code(to_f(u[e]), q) : (int8_t)0;
-    cr[j / V] = c;
+    for (int e = 0; e < V; ++e) f[e] = to_f(u[e]);
+    if (q.inv != 0.f) quant_codes<T, V>(f, q, w);
+    else
+#pragma unroll
+      for (int e = 0; e < (V + 3) / 4; ++e) w[e] = 0;
+    if constexpr (V == 8) *(uint2*)(cr + j / V) = make_uint2(w[0], w[1]);
+    else if constexpr (V == 4) *(uint32_t*)(cr + j / V) = w[0];
+    else if constexpr (V == 2) *(uint16_t*)(cr + j / V) = (uint16_t)w[0];
+    else *(uint8_t*)(cr + j / V) = (uint8_t)w[0];
   };
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if ((lane + i * G) * V < kpad) put(v[i], (lane + i * G) * V);
+    if ((lane + i * G) * V < kpad) put(v[i], (lane + i * G) * V);   // columns behind k: zeros
   for (int j = (lane + NV * G) * V; j < kpad; j += G * V) {
     Vec u{};
     if (j < k) u = *(const Vec*)(xr + j);
@@ -114,7 +177,7 @@ struct Int8Args {
   int64_t ldr1, ldy, ldx;
   int32_t m, n, k, kpad, act;
   float slope;
-  int32_t wide;   // y and r1 take 16-byte accesses at multiples of 16 columns, and the activation is not GELU
+  int32_t wide;   // y, r1, ws and bias take 16-byte accesses at multiples of 16 columns; not GELU
 };
 
 template <typename T>
@@ -126,57 +189,84 @@ __device__ __forceinline__ void int8_finish_one(const Int8Args& a, int64_t row, 
   ((T*)a.y)[row * a.ldy + col] = from_f<T>(u);
 }
 
-// N consecutive columns of one row, all inside y, aligned; not GELU.
+// N consecutive columns of one row, all inside y, aligned; not GELU.  ws, bias (or nullptr): those columns' own.
 template <typename T, int N>
-__device__ __forceinline__ void int8_finish(const Int8Args& a, int64_t row, int col, float xs, const int* acc) {
-  if (row >= a.m) return;
-  constexpr int E = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+struct Int8Out {
+  static constexpr int E = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
   typedef QuantVec<T, E> Vec;
-  T* y = (T*)a.y + row * a.ldy + col;
-  const T* r = (const T*)a.r1 + row * a.ldr1 + col;
+  Vec o[N / E];
+  __device__ __forceinline__ void compute(const Int8Args& a, int64_t row, int col, float xs, const int* acc,
+                                          const float* ws, const float* bias) {
+    float v[N];
+    floatx4 b[N / 4] = {};
+    if (bias)
 #pragma unroll
-  for (int e = 0; e < N; e += E) {
-    float v[E];
+      for (int e = 0; e < N / 4; ++e) b[e] = *(const floatx4*)(bias + 4 * e);
 #pragma unroll
-    for (int f = 0; f < E; ++f) v[f] = (float)acc[e + f] * (xs * a.ws[col + e + f]);
-    if (a.bias)
+    for (int e = 0; e < N / 4; ++e) {
+      const floatx4 w = *(const floatx4*)(ws + 4 * e);
 #pragma unroll
-      for (int f = 0; f < E; ++f) v[f] += a.bias[col + e + f];
-    if (a.act == LIC_ACT_RELU) {
+      for (int f = 0; f < 4; ++f) v[4 * e + f] = (float)acc[4 * e + f] * (xs * w[f]) + b[e][f];
+    }
+    if (a.act != LIC_ACT_NONE) {
+      const bool relu = a.act == LIC_ACT_RELU;
 #pragma unroll
-      for (int f = 0; f < E; ++f) v[f] = v[f] > 0.f ? v[f] : 0.f;
-    } else if (a.act == LIC_ACT_LRELU) {
-#pragma unroll
-      for (int f = 0; f < E; ++f) v[f] = v[f] > 0.f ? v[f] : v[f] * a.slope;
+      for (int e = 0; e < N; ++e) v[e] = v[e] > 0.f ? v[e] : (relu ? 0.f : v[e] * a.slope);
     }
     if (a.r1) {
-      const Vec u = *(const Vec*)(r + e);
+      const Vec* r = (const Vec*)((const T*)a.r1 + (row < a.m ? row : 0) * a.ldr1 + col);
 #pragma unroll
-      for (int f = 0; f < E; ++f) v[f] += to_f(u[f]);
+      for (int e = 0; e < N / E; ++e) {
+        const Vec u = r[e];
+#pragma unroll
+        for (int f = 0; f < E; ++f) v[E * e + f] += to_f(u[f]);
+      }
     }
-    Vec o;
 #pragma unroll
-    for (int f = 0; f < E; ++f) o[f] = from_f<T>(v[f]);
-    *(Vec*)(y + e) = o;
+    for (int e = 0; e < N / E; ++e) o[e] = __builtin_convertvector(*(QuantVec<float, E>*)(v + E * e), Vec);
   }
-}
+  __device__ __forceinline__ void store(const Int8Args& a, int64_t row, int col) const {
+    if (row >= a.m) return;
+    T* y = (T*)a.y + row * a.ldy + col;
+#pragma unroll
+    for (int e = 0; e < N / E; ++e) *(Vec*)(y + e * E) = o[e];
+  }
+};
 
-// A wave's 32 x 32 tile (lane: token lane & 31, channels 16 (lane / 32) ..): wide stores where the tile lies inside y, else
-// one element at a time through the wave's 4 KB of LDS.
+// A wave's 32 x 32 tile (lane: token m0 + lane % 32 with scale xs, channels n0 + 16 (lane / 32) ..): wide stores where the
+// tile lies inside y, else turned in the wave's LDS (INT8_STAGE words) so that 32 lanes meet consecutive channels.
+constexpr int INT8_STAGE = 32 * 33;
 template <typename T>
-__device__ __forceinline__ void int8_tile_out(const Int8Args& a, int64_t token, int n0, float xs, const int32x16& acc,
+__device__ __forceinline__ void int8_tile_out(const Int8Args& a, int64_t m0, int n0, float xs, const int32x16& acc,
                                               int* stage, int lane) {
+  const int row = lane & 31, half = lane >> 5;
   if (a.wide && n0 + 32 <= a.n) {
     int v[16];
+    const int col = n0 + 16 * half;
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = acc[e];
-    int8_finish<T, 16>(a, token, n0 + 16 * (lane >> 5), xs, v);
+    Int8Out<T, 16> out;
+    out.compute(a, m0 + row, col, xs, v, a.ws + col, a.bias ? a.bias + col : nullptr);
+    out.store(a, m0 + row, col);
     return;
   }
 #pragma unroll
-  for (int e = 0; e < 16; ++e) stage[e * 64 + lane] = acc[e];
-#pragma nounroll
-  for (int e = 0; e < 16; ++e) int8_finish_one<T>(a, token, n0 + 16 * (lane >> 5) + e, xs, stage[e * 64 + lane]);
+  for (int e = 0; e < 16; ++e) stage[row * 33 + 16 * half + e] = acc[e];
+  wave_lds_sync();
+  const int col = n0 + row, at = min(col, a.n - 1);
+  const float ws = a.ws[at], bias = a.bias ? a.bias[at] : 0.f;
+#pragma unroll 2
+  for (int e = 0; e < 32; e += 2) {
+    const int64_t token = m0 + e + half;
+    const float s = __shfl(xs, e + half);
+    if (token < a.m && col < a.n) {
+      float u = (float)stage[(e + half) * 33 + row] * (s * ws) + bias;
+      u = apply_act(u, a.act, a.slope);
+      if (a.r1) u += to_f(((const T*)a.r1)[token * a.ldr1 + col]);
+      ((T*)a.y)[token * a.ldy + col] = from_f<T>(u);
+    }
+  }
+  wave_lds_sync();
 }
 
 // A 32 x 32 tile of v_mfma_i32_32x32x32_i8 with weights as the first operand: lane l holds token l & 31 and result rows
@@ -228,47 +318,95 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
   const int row = lane & 31, sw = (lane >> 1) & 3, half = lane >> 5;
   const int8_t* wbase = smem + (wn * TN * 32 + row) * BK;
   const int8_t* xbase = smem + (BN + wm * TM * 32 + row) * BK;
-  for (int s = 0; s < steps; ++s) {
-    // step s has landed: at most the loads of the two steps behind it are under way
-    if (s + 2 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");
-    else if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  int32x4 fw[2][TN], fx[2][TM];   // the fragments of a step's two halves
+  auto read = [&](int s, int kk) {
+    const int off = (s % STAGES) * ROWS * BK, c = ((2 * kk + half) ^ sw) << 4;
+#pragma unroll
+    for (int i = 0; i < TN; ++i) fw[kk][i] = *(const int32x4*)(wbase + off + i * 32 * BK + c);
+#pragma unroll
+    for (int j = 0; j < TM; ++j) fx[kk][j] = *(const int32x4*)(xbase + off + j * 32 * BK + c);
+  };
+  auto multiply = [&](int kk, int j0, int j1) {
+#pragma unroll
+    for (int j = j0; j < j1; ++j)
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[kk][i], fx[kk][j], acc[i][j], 0, 0, 0);
+  };
+  // waits until step s has landed for every wave (behind it at most the loads of two more steps are under way), and until
+  // every wave has what it read so far, so that the step before may be overwritten
+  auto landed = [&](int s) {
+    if (s + 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
+    else if (s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + STAGES - 1 < steps) load(s + STAGES - 1);   // over step s - 1, which every wave has left
-    const int off = (s % STAGES) * ROWS * BK;
-    int32x4 fw[2][TN], fx[2][TM];
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const int c = ((2 * kk + half) ^ sw) << 4;
-#pragma unroll
-      for (int i = 0; i < TN; ++i) fw[kk][i] = *(const int32x4*)(wbase + off + i * 32 * BK + c);
-#pragma unroll
-      for (int j = 0; j < TM; ++j) fx[kk][j] = *(const int32x4*)(xbase + off + j * 32 * BK + c);
+  };
+  landed(0);
+  if (STAGES - 1 < steps) load(STAGES - 1);
+  read(0, 0);
+  for (int s = 0; s < steps; ++s) {
+    // each half's fragments are read under the other half's products (after the first of them, whose wait for its own
+    // fragments would else be one for both); the barrier stands between the halves
+    multiply(0, 0, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    read(s, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(0, 1, TM);
+    __builtin_amdgcn_sched_barrier(0);
+    if (s + 1 < steps) {
+      landed(s + 1);
+      if (s + STAGES < steps) load(s + STAGES);
+      read(s + 1, 0);
     }
-    __builtin_amdgcn_sched_barrier(0);   // all reads first: the second half's arrive under the first half's products
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int j = 0; j < TM; ++j)
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[kk][i], fx[kk][j], acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(1, 0, TM);
+    __builtin_amdgcn_sched_barrier(0);
   }
   __syncthreads();   // the steps' buffers become the waves' staging
-  int* stage = (int*)smem + wave * 1024;
+  int* stage = (int*)smem + wave * INT8_STAGE;
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
     const int64_t token = m0 + (wm * TM + j) * 32 + row;
     const float xs = token < a.m ? a.xs[token] : 0.f;
 #pragma unroll
     for (int i = 0; i < TN; ++i)
-      int8_tile_out<T>(a, token, n0 + (wn * TN + i) * 32, xs, acc[i][j], stage, lane);
+      int8_tile_out<T>(a, m0 + (wm * TM + j) * 32, n0 + (wn * TN + i) * 32, xs, acc[i][j], stage, lane);
   }
 }
 
-// Few tokens: 16 channels x 16 TT tokens a workgroup, its 8 waves on an eighth of k each (fragments straight from memory),
-// joined in LDS.  Bound by the weights' bytes, or by latency.
+// Joins the eighths of k that the waves of the two kernels below computed (lane: token lane % 16, channels 4 (lane / 16) ..)
+// and writes 16 channels x 16 TT tokens.
+template <typename T, int TT>
+__device__ __forceinline__ void int8_join(const Int8Args& a, int (*part)[TT][256], const int32x4* acc, int n0, int64_t m0,
+                                          const float* xscale) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int t = 0; t < TT; ++t) *(int32x4*)&part[wave][t][(lane & 15) * 16 + 4 * (lane >> 4)] = acc[t];
+  __syncthreads();
+  for (int i = threadIdx.x; i < TT * 64; i += 512) {
+    const int t = i >> 6, l = i & 63;
+    int32x4 v{};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v += *(const int32x4*)&part[k][t][l * 4];
+    const int64_t token = m0 + 16 * t + l / 4;
+    if (token >= a.m) continue;
+    const float xs = xscale[token];
+    const int u[4] = {v[0], v[1], v[2], v[3]};
+    const int col = n0 + 4 * (l & 3);
+    if (a.wide && n0 + 16 <= a.n) {
+      Int8Out<T, 4> out;
+      out.compute(a, token, col, xs, u, a.ws + col, a.bias ? a.bias + col : nullptr);
+      out.store(a, token, col);
+    } else {
+#pragma nounroll
+      for (int e = 0; e < 4; ++e) int8_finish_one<T>(a, token, col + e, xs, v[e]);
+    }
+  }
+}
+
+// Few tokens: 16 channels x 16 TT tokens a workgroup, its 8 waves on an eighth of k each, fragments straight from memory.
+// Bound by the weights' bytes, or by latency.
 template <typename T, int TT>
 __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
   __shared__ int part[8][TT][256];
@@ -282,8 +420,21 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
 #pragma unroll
   for (int t = 0; t < TT; ++t) x[t] = a.xc + min(m0 + 16 * t + row, (int64_t)a.m - 1) * a.kpad + 16 * q;
   int32x4 acc[TT] = {};
-#pragma unroll 4
-  for (int s = s0; s < s1; ++s) {
+  int s = s0;
+  for (; s + 4 <= s1; s += 4) {   // four steps' loads under way at once
+    int32x4 fw[4], fx[4][TT];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      fw[u] = *(const int32x4*)(w + 64 * (s + u));
+#pragma unroll
+      for (int t = 0; t < TT; ++t) fx[u][t] = *(const int32x4*)(x[t] + 64 * (s + u));
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], fx[u][t], acc[t], 0, 0, 0);
+  }
+  for (; s < s1; ++s) {
     const int32x4 fw = *(const int32x4*)(w + 64 * s);
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
@@ -291,22 +442,240 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
       acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw, fx, acc[t], 0, 0, 0);
     }
   }
-  // lane: token row, channels 4 q .. 4 q + 3
+  int8_join<T, TT>(a, part, acc, n0, m0, a.xs);
+}
+
+// One to ONE_TOKENS tokens in one launch: every workgroup quantises them into LDS, its first weights already under way.
+constexpr int ONE_TOKENS = 4, ONE_VECS = 2;   // a thread's part of a row: ONE_VECS loads of 16 bytes
+template <typename T> constexpr int one_max_k() { return 512 * ONE_VECS * 16 / (int)sizeof(T); }
+template <typename T>
+__global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
+  constexpr int V = 16 / sizeof(T);
+  typedef QuantVec<T, V> Vec;
+  __shared__ int part[8][1][256];
+  __shared__ uint32_t most[ONE_TOKENS][8];
+  __shared__ float scale[ONE_TOKENS];
+  extern __shared__ __attribute__((aligned(16))) int8_t codes[];   // [m][kpad]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = lane & 15, q = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int steps = a.kpad / 64, s0 = steps * wave / 8, s1 = steps * (wave + 1) / 8;
+  const int8_t* w = a.w + (int64_t)min(n0 + row, a.n - 1) * a.kpad + 16 * q;
+  int32x4 fw[8];
 #pragma unroll
-  for (int t = 0; t < TT; ++t) *(int32x4*)&part[wave][t][row * 16 + 4 * q] = acc[t];
+  for (int u = 0; u < 8; ++u)
+    if (s0 + u < s1) fw[u] = *(const int32x4*)(w + 64 * (s0 + u));
+  Vec v[ONE_TOKENS][ONE_VECS];
+#pragma unroll
+  for (int r = 0; r < ONE_TOKENS; ++r) {
+    if (r >= a.m) break;
+    QuantMax<T> top;
+#pragma unroll
+    for (int i = 0; i < ONE_VECS; ++i) {
+      const int j = (threadIdx.x + 512 * i) * V;
+      v[r][i] = Vec{};
+      if (j < a.k) v[r][i] = *(const Vec*)((const T*)a.x + r * a.ldx + j);
+      top.add(v[r][i]);
+    }
+    uint32_t bits = top.bits();
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint32_t other = __shfl_xor(bits, o);
+      bits = other > bits ? other : bits;
+    }
+    if (lane == 0) most[r][wave] = bits;
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < TT * 64; i += 512) {
-    const int t = i >> 6, l = i & 63;
-    int32x4 v{};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += *(const int32x4*)&part[k][t][l * 4];
-    const int64_t token = m0 + 16 * t + l / 4;
-    const float xs = token < a.m ? a.xs[token] : 0.f;
-    const int u[4] = {v[0], v[1], v[2], v[3]};
-    if (a.wide && n0 + 16 <= a.n) int8_finish<T, 4>(a, token, n0 + 4 * (l & 3), xs, u);
-    else
+  for (int r = 0; r < ONE_TOKENS; ++r) {
+    if (r >= a.m) break;
+    uint32_t bits = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) int8_finish_one<T>(a, token, n0 + 4 * (l & 3) + e, xs, u[e]);
+    for (int i = 0; i < 8; ++i) bits = most[r][i] > bits ? most[r][i] : bits;
+    const float top = QuantMax<T>::value(bits);
+    if (threadIdx.x == 0) scale[r] = top / 127.f;
+    const QuantRow qr = quant_row(top);
+#pragma unroll
+    for (int i = 0; i < ONE_VECS; ++i) {
+      const int j = (threadIdx.x + 512 * i) * V;
+      if (j < a.kpad) {
+        float f[V];
+        uint32_t c[V / 4] = {};
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = to_f(v[r][i][e]);
+        if (qr.inv != 0.f) quant_codes<T, V>(f, qr, c);
+#pragma unroll
+        for (int e = 0; e < V / 4; ++e) ((uint32_t*)(codes + r * a.kpad + j))[e] = c[e];
+      }
+    }
+  }
+  __syncthreads();
+  const int8_t* x = codes + min(row, a.m - 1) * a.kpad + 16 * q;
+  int32x4 acc[1] = {};
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    if (s0 + u < s1)
+      acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], *(const int32x4*)(x + 64 * (s0 + u)), acc[0], 0, 0, 0);
+  for (int s = s0 + 8; s < s1; ++s)
+    acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const int32x4*)(w + 64 * s), *(const int32x4*)(x + 64 * s), acc[0],
+                                                   0, 0, 0);
+  int8_join<T, 1>(a, part, acc, n0, 0, scale);
+}
+
+// Many tokens of few channels (kpad = 64 KS; whole tiles of y only: n a multiple of 32, a.wide): 32 tokens a wave, quantised straight into matrix operands that stay in
+// registers; the weights pass through LDS, 64 channels at a time, the next under way.  x is read once and y written once, the
+// codes never reach memory.  A weight row's 16-byte chunks are placed so that a fragment read meets every bank once: rows
+// advance by 16 KS of the 64 words, so chunk ^ swizzle(row) within 4, 8 or 16 chunks spreads those that coincide.
+template <int KS>
+__device__ __forceinline__ int int8_rows_swizzle(int r) {
+  return KS % 4 == 0 ? r & 15 : KS % 2 == 0 ? (r >> 1) & 7 : (r >> 2) & 3;
+}
+
+template <typename T, int KS>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (KS <= 3 ? 4 : 3) : (KS == 1 ? 4 : KS <= 3 ? 3 : 2)) void int8_rows_kernel(Int8Args a) {
+  constexpr int CK = 2 * KS, KP = 64 * KS, V = 16 / sizeof(T), L = 16 / V;   // products of 32 k; loads of 16 elements
+  constexpr bool HOLD = CK * 16 * sizeof(T) <= 256;                          // a lane's half row fits 64 registers
+  typedef QuantVec<T, V> Vec;
+  __shared__ __attribute__((aligned(1024))) int8_t smem[2][64 * KP];
+  __shared__ __attribute__((aligned(16))) float cols[2][2][64];   // the chunk's scales and biases
+  constexpr int LINE = 64 * sizeof(T) + 16;                       // a token's results of a chunk (fp32)
+  __shared__ __attribute__((aligned(16))) char stage[4][sizeof(T) == 2 ? 16 : 32 * LINE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = lane & 31, half = lane >> 5;
+  const int64_t token = (int64_t)blockIdx.x * 128 + wave * 32 + row;
+  // the workgroup's share of the 64-channel chunks
+  const int all = (a.n + 63) / 64, first = all * blockIdx.y / gridDim.y, chunks = all * (blockIdx.y + 1) / gridDim.y;
+
+  auto load = [&](int c) {
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      const int g = (wave * KS + j) * 64 + lane, r = g / (4 * KS), p = g % (4 * KS);
+      const int64_t ch = min(64 * c + int8_channel(r), a.n - 1);
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(a.w + ch * KP + 16 * (p ^ int8_rows_swizzle<KS>(r))),
+          (int8_lds_void*)(smem[c & 1] + (wave * KS + j) * 1024), 16, 0, 0);
+    }
+    const float* col = wave == 0 ? a.ws : wave == 1 ? a.bias : nullptr;
+    if (col)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(col + min(64 * c + lane, a.n - 1)),
+                                       (int8_lds_void*)cols[c & 1][wave], 4, 0, 0);
+  };
+  load(first);
+  if (!a.bias && threadIdx.x < 128) cols[threadIdx.x >> 6][1][lane] = 0.f;
+
+  const T* x = (const T*)a.x + min(token, (int64_t)a.m - 1) * a.ldx + 16 * half;
+  Vec raw[HOLD ? CK : 1][L];
+  QuantMax<T> most;
+  auto fetch = [&](int ks, Vec* u) {
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      u[l] = Vec{};
+      if (32 * ks + 16 * half + V * l < a.k) u[l] = *(const Vec*)(x + 32 * ks + V * l);
+    }
+  };
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int ks = 0; ks < CK; ++ks) fetch(ks, raw[ks]);
+  }
+#pragma unroll
+  for (int ks = 0; ks < CK; ++ks) {
+    Vec* u = raw[HOLD ? ks : 0];
+    if constexpr (!HOLD) fetch(ks, u);
+#pragma unroll
+    for (int l = 0; l < L; ++l) most.add(u[l]);
+  }
+  const uint32_t bits = most.bits(), other = __shfl_xor(bits, 32);
+  const float top = QuantMax<T>::value(other > bits ? other : bits);
+  const float xs = top / 127.f;
+  const QuantRow q = quant_row(top);
+  int32x4 fx[CK];
+#pragma unroll
+  for (int ks = 0; ks < CK; ++ks) {
+    Vec* u = raw[HOLD ? ks : 0];
+    if constexpr (!HOLD) fetch(ks, u);
+    float f[16];
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) f[e] = to_f(u[e / V][e % V]);
+    if (q.inv != 0.f) quant_codes<T, 16>(f, q, w);
+    fx[ks] = int32x4{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+  }
+
+  const int sw = int8_rows_swizzle<KS>(row);   // the same for both tiles: 32 rows apart
+  auto landed = [] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  landed();
+  if (first + 1 < chunks) load(first + 1);
+  for (int c = first; c < chunks; ++c) {
+    Int8Out<T, 16> out[2] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int32x16 acc{};
+#pragma unroll
+      for (int ks = 0; ks < CK; ++ks) {
+        const int32x4 fw = *(const int32x4*)(smem[c & 1] + (32 * i + row) * KP + 16 * ((2 * ks + half) ^ sw));
+        acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw, fx[ks], acc, 0, 0, 0);
+      }
+      const int at = 32 * i + 16 * half;
+      int v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = acc[e];
+      if (64 * c + 32 * i < a.n) out[i].compute(a, token, 64 * c + at, xs, v, cols[c & 1][0] + at, cols[c & 1][1] + at);
+    }
+    // chunk c + 1 has landed and chunk c been read by every wave; this chunk's stores come after the wait, so that they
+    // have a whole chunk's time until the next
+    landed();
+    if (c + 2 < chunks) load(c + 2);
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (64 * c + 32 * i < a.n) out[i].store(a, token, 64 * c + 32 * i + 16 * half);
+    } else {
+      // 64 bytes a lane would be four stores of a line's eighth each: through the wave's LDS, a store covers two lines of
+      // each of its tokens (131072 x 192 -> 576: 134.8 -> 94.9 us; 16-bit results gain nothing by it, 54.4 / 56.1)
+      char* st = stage[wave];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16 / V; ++e) *(Vec*)(st + row * LINE + (32 * i + 16 * half + V * e) * sizeof(T)) = out[i].o[e];
+      wave_lds_sync();
+      Vec u[32 / V];
+#pragma unroll
+      for (int e = 0; e < 32 / V; ++e)
+        u[e] = *(const Vec*)(st + (e * 64 + lane) / (64 / V) * LINE + (e * 64 + lane) % (64 / V) * 16);
+#pragma unroll
+      for (int e = 0; e < 32 / V; ++e) {
+        const int col = (e * 64 + lane) % (64 / V) * V;
+        const int64_t to = token - row + (e * 64 + lane) / (64 / V);
+        if (to < a.m && 64 * c + col < a.n) *(Vec*)((T*)a.y + to * a.ldy + 64 * c + col) = u[e];
+      }
+    }
+  }
+}
+
+constexpr int ROWS_FILL = 512;   // workgroups; 32768 x 192 -> 576 fp16: 28.0 us with 256, 23.5 with 512, 24.8 with 1024
+template <typename T, int KS>
+static int rows_launch(const Int8Args& a, hipStream_t s) {
+  // channels are shared out where the token blocks alone would not fill the chip (each share quantises its tokens again)
+  const int blocks = (int)(((int64_t)a.m + 127) / 128), chunks = (a.n + 63) / 64;
+  const int shares = blocks >= ROWS_FILL ? 1 : (ROWS_FILL + blocks - 1) / blocks < chunks ? (ROWS_FILL + blocks - 1) / blocks : chunks;
+  hipLaunchKernelGGL((int8_rows_kernel<T, KS>), dim3((unsigned)blocks, (unsigned)shares), dim3(256), 0, s, a);
+  LIC_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
+static int rows_run(const Int8Args& a, hipStream_t s) {
+  switch (a.kpad / 64) {
+    case 1: return rows_launch<T, 1>(a, s);
+    case 2: return rows_launch<T, 2>(a, s);
+    case 3: return rows_launch<T, 3>(a, s);
+    case 4: return rows_launch<T, 4>(a, s);
+    case 5: return rows_launch<T, 5>(a, s);
+    case 6: return rows_launch<T, 6>(a, s);
+    default: return fail("linear_int8: rows kernel sizes");
   }
 }
 
@@ -317,7 +686,6 @@ static void quantize_launch(const void* x, int64_t ldx, int m, int k, int8_t* co
   // lanes of a row: up to four vectors each, a whole wave from there on
   if (vecs <= 32) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 8>), dim3((m + 31) / 32), dim3(256), 0, s, (const T*)x, ldx, m, k, codes, kpad, scale);
   else if (vecs <= 64) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 16>), dim3((m + 15) / 16), dim3(256), 0, s, (const T*)x, ldx, m, k, codes, kpad, scale);
-  else if (vecs <= 1024) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 64>), dim3((m + 3) / 4), dim3(256), 0, s, (const T*)x, ldx, m, k, codes, kpad, scale);
   else hipLaunchKernelGGL((quantize_int8_kernel<T, V, 64>), dim3((m + 3) / 4), dim3(256), 0, s, (const T*)x, ldx, m, k, codes, kpad, scale);
 }
 
@@ -362,10 +730,27 @@ static int few_launch(const Int8Args& a, hipStream_t s) {
 }
 
 template <typename T>
-static int linear_run(Int8Args a, hipStream_t s) {
-  const uintptr_t p = (uintptr_t)a.y | (uintptr_t)a.r1;
+static int one_launch(const Int8Args& a, hipStream_t s) {
+  hipLaunchKernelGGL(int8_one_kernel<T>, dim3((a.n + 15) / 16), dim3(512), a.m * a.kpad, s, a);
+  LIC_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
+static int linear_run(Int8Args a, int8_t* codes, float* scale, hipStream_t s) {
+  const uintptr_t p = (uintptr_t)a.y | (uintptr_t)a.r1 | (uintptr_t)a.ws | (uintptr_t)a.bias;
   constexpr int E = 16 / sizeof(T);
   a.wide = a.act != LIC_ACT_GELU && p % 16 == 0 && a.ldy % E == 0 && (!a.r1 || a.ldr1 % E == 0);
+  if (a.x) {
+    const bool aligned = (uintptr_t)a.x % 16 == 0 && a.ldx % E == 0 && a.k % E == 0;
+    if (aligned && a.m <= ONE_TOKENS && a.kpad <= one_max_k<T>()) return one_launch<T>(a, s);
+    // us, 192 -> 576 fp16 (quantised apart, tiles): 131072 tokens 54.4 (97), 16384: 16.0 (20.1), 8192: 13.4 (14.5), 4096: 12
+    // (10); 384 -> 384: 79.5 (94); from kpad 448 on the operands spill; fp32, 192 -> 576: 32768 tokens 34 (45), 8192: 21 (17.5)
+    if (aligned && a.m >= (sizeof(T) == 2 ? 8192 : 16384) && a.kpad <= 384 && a.wide && a.n % 32 == 0) return rows_run<T>(a, s);
+    if (quantize_run<T>(a.x, a.ldx, a.m, a.k, codes, a.kpad, scale, s)) return 1;
+    a.xc = codes;
+    a.xs = scale;
+  }
   if (a.m <= 16) return few_launch<T, 1>(a, s);
   if (a.m <= 64) return few_launch<T, 4>(a, s);
   const int64_t big = ((int64_t)a.m + 255) / 256 * ((a.n + 255) / 256);
@@ -417,14 +802,11 @@ extern "C" int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const 
     if (ldx < k) return fail("linear_int8: row stride below k");
     if (!ws || (uintptr_t)ws % 16 || ws_bytes < lic_linear_int8_workspace(m, kpad))
       return fail("linear_int8: workspace missing, misaligned or too small");
-    int8_t* codes = (int8_t*)ws;
-    float* scale = (float*)((char*)ws + ((int64_t)m * kpad + 15) / 16 * 16);
-    if (quantize_any(dtype, x, ldx, m, k, codes, kpad, scale, s)) return 1;
-    xcodes = codes;
-    xscale = scale;
   }
   Int8Args a{xcodes, xscale, w, wscale, bias, r1, y, x, ldr1, ldy, ldx, m, n, k, kpad, act, slope, 0};
-  if (dtype == LIC_F32) return linear_run<float>(a, s);
-  if (dtype == LIC_F16) return linear_run<half_t>(a, s);
-  return linear_run<bf16_t>(a, s);
+  int8_t* codes = (int8_t*)ws;
+  float* scale = (float*)((char*)ws + ((int64_t)m * kpad + 15) / 16 * 16);
+  if (dtype == LIC_F32) return linear_run<float>(a, codes, scale, s);
+  if (dtype == LIC_F16) return linear_run<half_t>(a, codes, scale, s);
+  return linear_run<bf16_t>(a, codes, scale, s);
 }

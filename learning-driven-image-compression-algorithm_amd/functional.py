@@ -1242,37 +1242,42 @@ def linear_int8(x, pk: Int8Pack, out: Optional[Act] = None, *, act: int = _ffi.A
     """act(x W^T + bias) + r1 per token of x (an Act, quantised by the call, or an Int8Act) in 8-bit products: integer
     sums, so equal codes give equal results whatever the batch, the tile or the device.  Forward only."""
     q = x if isinstance(x, Int8Act) else None
-    B, H, W = q.shape if q is not None else (x.B, x.H, x.W)
     src = q.codes if q is not None else x.t
+    B, H, W, _ = src.shape
+    dtype, co, r1t = x.dtype, pk.w.shape[0], r1.t if r1 is not None else None
     if x.c != pk.ci:
         raise ValueError(f"linear_int8: input has {x.c} channels, weights expect {pk.ci}")
-    _on_current_device("linear_int8", src, pk.w, r1.t if r1 is not None else None, out.t if out is not None else None)
-    if act not in (_ffi.ACT_NONE, _ffi.ACT_RELU, _ffi.ACT_LRELU, _ffi.ACT_GELU):
+    _on_current_device("linear_int8", src, pk.w, r1t)
+    if act not in _INT8_ACTS:
         raise ValueError("linear_int8: act must be ACT_NONE, ACT_RELU, ACT_LRELU or ACT_GELU")
+    given = out
     if out is None:
-        out = Act.empty(B, H, W, pk.co, x.dtype, src.device)
-    for v, what in ((out, "out"), (r1, "r1")):
-        if v is not None and ((v.B, v.H, v.W, v.c) != (B, H, W, pk.co) or v.dtype != x.dtype):
-            raise ValueError(f"linear_int8: {what} must be a {x.dtype} view of {(B, H, W, pk.co)}")
-    if q is None and _overlaps(x, out):
-        raise ValueError("linear_int8: out overlaps x")
-    if r1 is not None and (r1.ptr != out.ptr or r1.ld != out.ld) and _overlaps(r1, out):
-        raise ValueError("linear_int8: out overlaps r1 (only r1 itself may be written)")
+        out = Act(torch.empty((B, H, W, co), dtype=dtype, device=src.device))
+    for v, what in ((given, "out"), (r1, "r1")):
+        if v is not None and ((v.B, v.H, v.W, v.c) != (B, H, W, co) or v.dtype != dtype):
+            raise ValueError(f"linear_int8: {what} must be a {dtype} view of {(B, H, W, co)}")
+    if given is not None:
+        _on_current_device("linear_int8", out.t)
+        if q is None and _overlaps(x, out):
+            raise ValueError("linear_int8: out overlaps x")
+        if r1 is not None and (r1.ptr != out.ptr or r1.ld != out.ld) and _overlaps(r1, out):
+            raise ValueError("linear_int8: out overlaps r1 (only r1 itself may be written)")
     m, kpad = B * H * W, pk.w.shape[1]
     if m == 0:
         return out
-    lib = _lib()
-    ws, nbytes = None, 0
-    if q is None:
-        nbytes = int(lib.lic_linear_int8_workspace(m, kpad))
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=src.device)
+    nbytes = 0 if q is not None else -(-m * kpad // 16) * 16 + 4 * m      # lic_linear_int8_workspace
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=src.device) if nbytes else None
     r1p, ldr1 = _ptr(r1)
-    check(lib.lic_linear_int8(dtype_id(x.dtype), None if q is not None else x.ptr, 0 if q is not None else x.ld,
-                              _dp(q.codes) if q is not None else None, _dp(q.scale) if q is not None else None,
-                              m, pk.ci, _dp(pk.w), kpad, _dp(pk.scale), _dp(pk.bias) if pk.bias is not None else None,
-                              pk.co, act, slope, r1p, ldr1, out.ptr, out.ld, _dp(ws) if ws is not None else None,
-                              nbytes, stream_handle()))
+    check(_lib().lic_linear_int8(dtype_id(dtype), None if q is not None else x.ptr, 0 if q is not None else x.ld,
+                                 src.data_ptr() if q is not None else None,
+                                 _dp(q.scale) if q is not None else None, m, pk.ci, pk.w.data_ptr(), kpad,
+                                 _dp(pk.scale), _dp(pk.bias) if pk.bias is not None else None, co, act, slope, r1p,
+                                 ldr1, out.ptr, out.t.shape[3], ws.data_ptr() if nbytes else None, nbytes,
+                                 stream_handle()))
     return out
+
+
+_INT8_ACTS = (_ffi.ACT_NONE, _ffi.ACT_RELU, _ffi.ACT_LRELU, _ffi.ACT_GELU)
 
 
 def int8_mode() -> bool:
