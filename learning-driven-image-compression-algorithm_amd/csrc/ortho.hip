@@ -1,198 +1,482 @@
 // Newton-Schulz orthogonalisation of many matrices at once (gfx950):
 //   X = G / (|G|_F + eps);  `steps` times: A = X X^T, X = (a I + b A + c A A) X
 // on r x c matrices with r <= c (G^T where G has more rows than columns).
+//
+// Every product runs on fp16 matrix instructions with operands of two parts, value = hi + lo (22 bits), as
+// hi hi' + hi lo' + lo hi' with fp32 sums: the error of fp32 products at three eighths of their cost (one part alone would
+// leave 4e-4 .. 3e-3 of the result, two parts leave what fp32 leaves, 2e-6 at 192 x 1728).  X is held divided by a power of
+// two above its norm (from |G| and the polynomial's bounds), so the parts never leave fp16's range.
+//
+// Operands lie in fragment order: [row / 32][k / 16][hi, lo][64 lanes][8], one contiguous KB a fragment, loaded straight into
+// registers; place p of a 32-row tile is row 16 ((p / 4) % 2) + 4 (p / 8) + p % 4 of it.  With that order on both operands a
+// lane's 16 results (rows 8 (i / 4) + 4 (lane / 32) + i % 4 of the instruction) are 16 consecutive rows, a whole k step of the
+// transposed operand.  X is kept in both orders: rows along r for A = X X^T, rows along c (X^T) for Q X.
 #include "lic_common.h"
+#include <cmath>
 
 namespace lic {
+
+constexpr int ORTHO_MAX_STEPS = 64;
 
 struct OrthoDesc {
   const void* g;
   void* out;
   int64_t rs, cs;       // strides of G's (or G^T's) rows and columns
-  int64_t x0, x1;       // the two copies of X, floats from the workspace's float area
-  int64_t a, q;         // A and Q = a I + b A + c A A
+  int64_t x, xt;        // the two copies of X in both orders, halves from the workspace's operand area; the second of
+  int64_t a, q;         // each follows at + step.  A and Q = a I + b A + c A A
+  int64_t step;
   int32_t r, c, flip;   // flip: out is the transpose of X
-  int32_t norm0;        // first partial sum of |G|^2
-  int32_t gram0, upd0;  // first block of the r x r and of the r x c tiles
+  int32_t parts0;       // first of its 64 x 64 tiles' partial sums of |G|^2
+  int32_t gram0, upd0;  // first workgroup of A's lower triangle, and of X
 };
 
-constexpr int ORTHO_BATCH = 32;   // descriptors a launch carries to the device in its arguments
+// The workgroups of a stage in matrix order.
+struct OrthoTile { int32_t mat, at; };
+
+constexpr int ORTHO_BATCH = 24;   // descriptors that a launch carries to the device in its arguments
 struct OrthoBatch { OrthoDesc d[ORTHO_BATCH]; };
 
-__global__ void ortho_desc_kernel(OrthoBatch b, int first, int count, OrthoDesc* dst) {
-  if ((int)threadIdx.x < count) dst[first + threadIdx.x] = b.d[threadIdx.x];
+struct OrthoWork {
+  OrthoDesc* desc;
+  OrthoTile *tiles, *gram, *upd;   // 64 x 64 tiles of G, lower tiles of A, 64 x 256 tiles of X
+  double* parts;
+  int32_t* exps;                   // [count][ORTHO_MAX_STEPS + 1] exponents of X's scale
+  half_t* ops;
+};
+
+// What the polynomial alone says: bounds of |X| after k steps for |X| <= 1, of |X'| / |X|, exponents of Q's scale.
+struct OrthoBounds {
+  float most[ORTHO_MAX_STEPS + 1], gain;
+  int32_t qexp[ORTHO_MAX_STEPS];
+};
+
+__device__ __forceinline__ int ortho_tiles(int n) { return (n + 63) / 64; }
+
+__global__ __launch_bounds__(256) void ortho_setup_kernel(OrthoBatch b, int first, OrthoWork w) {
+  const OrthoDesc d = b.d[blockIdx.x];
+  const int mat = first + blockIdx.x, nr = ortho_tiles(d.r), nc = ortho_tiles(d.c), nu = (d.c + 255) / 256;
+  if (threadIdx.x == 0) w.desc[mat] = d;
+  for (int i = threadIdx.x; i < nr * nc; i += 256) w.tiles[d.parts0 + i] = {mat, i};
+  for (int i = threadIdx.x; i < nr * nu; i += 256) w.upd[d.upd0 + i] = {mat, i};
+  for (int i = threadIdx.x; i < nr; i += 256)
+    for (int j = 0; j <= i; ++j) w.gram[d.gram0 + i * (i + 1) / 2 + j] = {mat, i << 16 | j};
 }
 
-template <int OrthoDesc::* FIRST>
-__device__ __forceinline__ int ortho_find(const OrthoDesc* d, int count, int block) {
-  int lo = 0, hi = count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (d[mid].*FIRST <= block) lo = mid;
-    else hi = mid - 1;
+// Workgroups go round the 8 XCDs: a run of neighbouring tiles for each, which share operands in its L2.
+__device__ __forceinline__ int ortho_id() {
+  const int n = gridDim.x, xcd = blockIdx.x & 7, per = n >> 3, more = n & 7;
+  return xcd * per + min(xcd, more) + (int)(blockIdx.x >> 3);
+}
+
+__device__ __forceinline__ int ortho_place(int p) { return (((p >> 2) & 1) << 4) | (((p >> 3) & 3) << 2) | (p & 3); }
+
+// A 64 x 64 tile of G, element (i, j) of it to thread (of 256) and slot (of 16) so that either order of G reads in lines.
+template <typename T, typename F>
+__device__ __forceinline__ void ortho_read(const OrthoDesc& d, int i0, int j0, F f) {
+  const bool along = d.cs <= d.rs;   // columns are the nearer ones
+  const int fast = threadIdx.x & 63, slow = threadIdx.x >> 6;
+#pragma unroll 4
+  for (int s = 0; s < 16; ++s) {
+    const int i = along ? slow * 16 + s : fast, j = along ? fast : slow * 16 + s;
+    const bool in = i0 + i < d.r && j0 + j < d.c;
+    f(i, j, in ? to_f(((const T*)d.g)[(i0 + i) * d.rs + (j0 + j) * d.cs]) : 0.f);
   }
-  return lo;
 }
 
-constexpr int ORTHO_NORM = 4096;   // elements of one partial sum
-
-// Partial sums of squares in 64 bits: small gradients square to below fp32's range.
+// Sums of squares in 64 bits: the squares of small gradients are below fp32's range.
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_norm_kernel(const OrthoDesc* desc, int count, double* parts) {
+__global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoWork w) {
   __shared__ double red[4];
-  const int i = ortho_find<&OrthoDesc::norm0>(desc, count, blockIdx.x);
-  const OrthoDesc d = desc[i];
-  const int64_t first = (int64_t)((int)blockIdx.x - d.norm0) * ORTHO_NORM, total = (int64_t)d.r * d.c;
+  const OrthoTile t = w.tiles[blockIdx.x];
+  const OrthoDesc d = w.desc[t.mat];
+  const int nc = ortho_tiles(d.c);
   double s = 0;
-  for (int64_t e = first + threadIdx.x; e < first + ORTHO_NORM && e < total; e += 256) {
-    const double v = (double)to_f(((const T*)d.g)[e / d.c * d.rs + e % d.c * d.cs]);
-    s += v * v;
-  }
+  ortho_read<T>(d, t.at / nc * 64, t.at % nc * 64, [&](int, int, float v) { s += (double)v * (double)v; });
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) parts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+  if (threadIdx.x == 0) w.parts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
+// value * 2^14 in two fp16 parts (|value| <= 1)
+struct OrthoParts { half8 hi, lo; };
+__device__ __forceinline__ void ortho_split(OrthoParts& p, int e, float scaled) {
+  const half_t h = (half_t)scaled;
+  p.hi[e] = h;
+  p.lo[e] = (half_t)(scaled - (float)h);
+}
+
+// The fragments of a 64 x 64 tile in LDS (t[row][col], `flip`: its transpose): thread (of 512) -> 8 values of k.
+constexpr int ORTHO_LD = 65;
+template <bool FLIP>
+__device__ __forceinline__ OrthoParts ortho_gather(const float* t, int rowtile, int ks, int lane, float scale) {
+  const int row = 32 * rowtile + ortho_place(lane & 31), k = 16 * ks + 8 * (lane >> 5);
+  OrthoParts p;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ortho_split(p, e, scale * (FLIP ? t[(k + e) * ORTHO_LD + row] : t[row * ORTHO_LD + k + e]));
+  return p;
+}
+__device__ __forceinline__ half_t* ortho_fragment(half_t* m, int ksteps, int rowtile, int ks) {
+  return m + ((int64_t)rowtile * ksteps + ks) * 1024;
+}
+__device__ __forceinline__ void ortho_put(half_t* frag, int lane, const OrthoParts& p) {
+  *(half8*)(frag + lane * 8) = p.hi;
+  *(half8*)(frag + 512 + lane * 8) = p.lo;
+}
+
+// X = G / (|G| + eps) in both orders; the exponents of all steps' scales.
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_scale_kernel(const OrthoDesc* desc, int count, const double* parts,
-                                                          float eps, float* f) {
-  const int i = ortho_find<&OrthoDesc::norm0>(desc, count, blockIdx.x);
-  const OrthoDesc d = desc[i];
-  const int64_t first = (int64_t)((int)blockIdx.x - d.norm0) * ORTHO_NORM, total = (int64_t)d.r * d.c;
+__global__ __launch_bounds__(256) void ortho_scale_kernel(OrthoWork w, OrthoBounds b, int steps, float eps) {
+  __shared__ double red[4];
+  __shared__ float tile[64 * ORTHO_LD];
+  const OrthoTile t = w.tiles[blockIdx.x];
+  const OrthoDesc d = w.desc[t.mat];
+  const int nr = ortho_tiles(d.r), nc = ortho_tiles(d.c), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   double s = 0;
-  for (int64_t p = 0; p * ORTHO_NORM < total; ++p) s += parts[d.norm0 + p];
-  const double inv = 1.0 / (sqrt(s) + (double)eps);
-  for (int64_t e = first + threadIdx.x; e < first + ORTHO_NORM && e < total; e += 256)
-    f[d.x0 + e] = (float)((double)to_f(((const T*)d.g)[e / d.c * d.rs + e % d.c * d.cs]) * inv);
-}
-
-// One 32 x 32 tile of P R (or P R^T) in fp32, four outputs a thread.
-template <bool TRANS>
-__device__ __forceinline__ void ortho_tile(const float* p, int ldp, const float* rr, int ldr, int rows, int cols,
-                                           int kk, int i0, int j0, float* acc) {
-  __shared__ float sp[32][33], sr[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  for (int k0 = 0; k0 < kk; k0 += 32) {
-    for (int q = ty; q < 32; q += 8) {
-      sp[q][tx] = (i0 + q < rows && k0 + tx < kk) ? p[(int64_t)(i0 + q) * ldp + k0 + tx] : 0.f;
-      if (TRANS) sr[tx][q] = (j0 + q < cols && k0 + tx < kk) ? rr[(int64_t)(j0 + q) * ldr + k0 + tx] : 0.f;
-      else sr[q][tx] = (k0 + q < kk && j0 + tx < cols) ? rr[(int64_t)(k0 + q) * ldr + j0 + tx] : 0.f;
+  for (int i = threadIdx.x; i < nr * nc; i += 256) s += w.parts[d.parts0 + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  const double norm = sqrt(red[0] + red[1] + red[2] + red[3]);
+  const double size = norm + (double)eps, ratio = size > 0 ? norm / size : 0.0;   // |X|
+  auto exponent = [](double v) {   // 2^e > v; bounded: below it X is zero in fp32
+    int e = 0;
+    if (v > 0 && v < 1e30) (void)frexp(v, &e);
+    return v > 0 ? (e > -140 ? e : -140) : -140;
+  };
+  const int e0 = norm == norm ? exponent(ratio) : 0;
+  if (t.at == 0 && threadIdx.x == 0) {
+    double most = ratio;
+    for (int k = 0; k <= steps; ++k) {
+      w.exps[t.mat * (ORTHO_MAX_STEPS + 1) + k] = norm == norm ? exponent(most) : 0;
+      most = fmin(most * (double)b.gain, (double)b.most[k < steps ? k + 1 : k]);
     }
-    __syncthreads();
-    float part[4] = {0, 0, 0, 0};   // sums of sums: a long row's rounding errors do not pile up
-    for (int k = 0; k < 32; ++k)
+  }
+  const double inv = size > 0 ? ldexp(1.0 / size, 14 - e0) : 0.0;
+  const int i0 = t.at / nc, j0 = t.at % nc;
+  ortho_read<T>(d, i0 * 64, j0 * 64, [&](int i, int j, float v) { tile[i * ORTHO_LD + j] = (float)((double)v * inv); });
+  __syncthreads();
+  half_t *x = w.ops + d.x, *xt = w.ops + d.xt;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) part[q] += sp[ty + 8 * q][k] * sr[k][tx];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) acc[q] += part[q];
-    __syncthreads();
+  for (int u = 0; u < 2; ++u) {
+    const int f = wave * 2 + u, rt = f >> 2, ks = f & 3;
+    ortho_put(ortho_fragment(x, nc * 4, i0 * 2 + rt, j0 * 4 + ks), lane, ortho_gather<false>(tile, rt, ks, lane, 1.f));
+    ortho_put(ortho_fragment(xt, nr * 4, j0 * 2 + rt, i0 * 4 + ks), lane, ortho_gather<true>(tile, rt, ks, lane, 1.f));
   }
 }
 
-// stage 0: A = X X^T;  1: Q = a I + b A + c A A
-__global__ __launch_bounds__(256) void ortho_gram_kernel(const OrthoDesc* desc, int count, float* f, int odd, int stage,
-                                                         float ca, float cb, float cc) {
-  const OrthoDesc d = desc[ortho_find<&OrthoDesc::gram0>(desc, count, blockIdx.x)];
-  const int nt = (d.r + 31) / 32, t = blockIdx.x - d.gram0;
-  const int i0 = t / nt * 32, j0 = t % nt * 32;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  float acc[4] = {0, 0, 0, 0};
-  const float* x = f + (odd ? d.x1 : d.x0);
-  if (stage == 0) ortho_tile<true>(x, d.c, x, d.c, d.r, d.r, d.c, i0, j0, acc);
-  else ortho_tile<true>(f + d.a, d.r, f + d.a, d.r, d.r, d.r, d.r, i0, j0, acc);
+// 64 x 64 results of P R^T over k steps [s0, s1), operands in fragment order (two row tiles each): acc[i][j] is P's tile i
+// against R's tile j.
+// Steps that the matrix instructions sum up before the rounded fp32 addition to the total: their own additions of a long chain
+// lose more.  2-norm error at 2048 x 2048: one chain 8.9e-6, chains of 16 steps 4.0e-6, of 8 3.3e-6, of 4 3.1e-6 (fp32
+// products: 5.6e-6); 128 x 576: 2.9e-6, .., 2.6e-6 (2.2e-6).  4 costs 1 to 3 % of the time.
+constexpr int ORTHO_CHAIN = 4;
+struct OrthoFrags { half8 p[2][2], r[2][2]; };
+__device__ __forceinline__ void ortho_load(OrthoFrags& f, const half_t* p, const half_t* r, int64_t ptile, int64_t rtile,
+                                           int s) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int i = i0 + ty + 8 * q, j = j0 + tx;
-    if (i >= d.r || j >= d.r) continue;
-    const int64_t at = (int64_t)i * d.r + j;
-    if (stage == 0) f[d.a + at] = acc[q];
-    else f[d.q + at] = (i == j ? ca : 0.f) + cb * f[d.a + at] + cc * acc[q];
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f.p[i][h] = *(const half8*)(p + i * ptile + (int64_t)s * 1024 + h * 512);
+      f.r[i][h] = *(const half8*)(r + i * rtile + (int64_t)s * 1024 + h * 512);
+    }
+}
+__device__ __forceinline__ void ortho_multiply(floatx16 (&acc)[2][2], const OrthoFrags& f) {
+#pragma unroll
+  for (int q = 0; q < 3; ++q)   // hi hi, hi lo, lo hi
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.p[i][q == 2], f.r[j][q == 1], acc[i][j], 0, 0, 0);
+}
+__device__ __forceinline__ void ortho_product(floatx16 (&sum)[2][2], const half_t* p, const half_t* r, int64_t ptile,
+                                              int64_t rtile, int s0, int s1) {
+  if (s0 >= s1) return;
+  OrthoFrags f0, f1;   // one step is multiplied while the next one is under way
+  ortho_load(f0, p, r, ptile, rtile, s0);
+  for (int s = s0; s < s1;) {
+    floatx16 acc[2][2] = {};
+    const int end = s + ORTHO_CHAIN < s1 ? s + ORTHO_CHAIN : s1;
+    for (; s + 2 <= end; s += 2) {
+      ortho_load(f1, p, r, ptile, rtile, s + 1);
+      ortho_multiply(acc, f0);
+      ortho_load(f0, p, r, ptile, rtile, s + 2 < s1 ? s + 2 : s);
+      ortho_multiply(acc, f1);
+    }
+    if (s < end) {   // the last step of all
+      ortho_multiply(acc, f0);
+      ++s;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum[i][j][e] += acc[i][j][e];
   }
 }
 
-// X <- Q X; the last step writes the result
+// A = X X^T (STAGE 0), or Q = a I + b A + c A A (STAGE 1): a 64 x 64 tile of the lower triangle a workgroup, mirrored.  The 8
+// waves take an eighth of k each and are joined in LDS in a fixed order: a single long matrix has few tiles.
+template <int STAGE>
+__global__ __launch_bounds__(512) void ortho_gram_kernel(OrthoWork w, int k, int steps, float ca, float cb, float cc, int qexp) {
+  __shared__ float join[4][4096];   // [wave][tile of 32 x 32][result][lane]; then the tile, [64][ORTHO_LD]
+  const OrthoTile t = w.gram[ortho_id()];
+  const OrthoDesc d = w.desc[t.mat];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ti = t.at >> 16, tj = t.at & 0xffff, nr = ortho_tiles(d.r), nc = ortho_tiles(d.c);
+  const half_t* op = w.ops + (STAGE == 0 ? d.x + (k & 1) * d.step : d.a);
+  const int ksteps = (STAGE == 0 ? nc : nr) * 4;
+  const int64_t tile = (int64_t)ksteps * 1024;
+  floatx16 acc[2][2] = {};
+  ortho_product(acc, op + ti * 2 * tile + lane * 8, op + tj * 2 * tile + lane * 8, tile, tile, ksteps * wave / 8,
+                ksteps * (wave + 1) / 8);
+  if (wave >= 4) {
+#pragma unroll
+    for (int e = 0; e < 64; ++e) join[wave - 4][e * 64 + lane] = acc[e >> 5][(e >> 4) & 1][e & 15];
+  }
+  __syncthreads();
+  if (wave < 4) {
+#pragma unroll
+    for (int e = 0; e < 64; ++e) join[wave][e * 64 + lane] += acc[e >> 5][(e >> 4) & 1][e & 15];
+  }
+  __syncthreads();
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int at = e * 512 + threadIdx.x;
+    v[e] = (join[0][at] + join[1][at]) + (join[2][at] + join[3][at]);
+  }
+  __syncthreads();
+  float* out = &join[0][0];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int at = e * 512 + threadIdx.x, l = at & 63, f = at >> 6, i = f & 15, b = (f >> 4) & 1, a = f >> 5;
+    out[(32 * a + 16 * (l >> 5) + i) * ORTHO_LD + 32 * b + ortho_place(l & 31)] = v[e];
+  }
+  __syncthreads();
+  // a fragment a wave, and the mirrored tile's
+  const int rt = wave >> 2, ks = wave & 3;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    if (m == 1 && ti == tj) break;
+    const int I = m ? tj : ti, J = m ? ti : tj;
+    // the sum carries 2^28
+    OrthoParts p;
+    if constexpr (STAGE == 0) {
+      p = m ? ortho_gather<true>(out, rt, ks, lane, 0x1p-14f) : ortho_gather<false>(out, rt, ks, lane, 0x1p-14f);
+      ortho_put(ortho_fragment(w.ops + d.a, nr * 4, I * 2 + rt, J * 4 + ks), lane, p);
+    } else {
+      const half_t* f = ortho_fragment(w.ops + d.a, nr * 4, I * 2 + rt, J * 4 + ks);
+      const half8 hi = *(const half8*)(f + lane * 8), lo = *(const half8*)(f + 512 + lane * 8);
+      const int e2 = 2 * w.exps[t.mat * (ORTHO_MAX_STEPS + 1) + k];
+      const float s1 = ldexpf(cb, e2 - 14), s2 = ldexpf(cc, 2 * e2 - 28), down = ldexpf(1.f, 14 - qexp);
+      const int row = 32 * rt + ortho_place(lane & 31), col = 16 * ks + 8 * (lane >> 5);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float aa = m ? out[(col + e) * ORTHO_LD + row] : out[row * ORTHO_LD + col + e];
+        float v = s1 * ((float)hi[e] + (float)lo[e]) + s2 * aa;
+        if (I * 64 + row == J * 64 + col + e) v += ca;
+        ortho_split(p, e, down * v);
+      }
+      ortho_put(ortho_fragment(w.ops + d.q, nr * 4, I * 2 + rt, J * 4 + ks), lane, p);
+    }
+  }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void ortho_out(T* out, int count, bool wide, const float* v) {
+  if (wide && count >= N) {
+    constexpr int E = 16 / sizeof(T);
+    typedef T Vec __attribute__((ext_vector_type(E)));
+#pragma unroll
+    for (int e = 0; e < N; e += E) {
+      Vec o;
+#pragma unroll
+      for (int f = 0; f < E; ++f) o[f] = from_f<T>(v[e + f]);
+      *(Vec*)(out + e) = o;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < count) out[e] = from_f<T>(v[e]);
+  }
+}
+
+// X <- Q X: 64 rows x 64 columns a wave, 64 x 256 a workgroup (Q's fragments are shared through the L1).  The last step
+// writes the result instead.
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_update_kernel(const OrthoDesc* desc, int count, float* f, int odd,
-                                                           int last) {
-  const OrthoDesc d = desc[ortho_find<&OrthoDesc::upd0>(desc, count, blockIdx.x)];
-  const int nt = (d.c + 31) / 32, t = blockIdx.x - d.upd0;
-  const int i0 = t / nt * 32, j0 = t % nt * 32;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  float acc[4] = {0, 0, 0, 0};
-  ortho_tile<false>(f + d.q, d.r, f + (odd ? d.x1 : d.x0), d.c, d.r, d.c, d.r, i0, j0, acc);
-  float* xn = f + (odd ? d.x0 : d.x1);
+__global__ __launch_bounds__(256) void ortho_update_kernel(OrthoWork w, int k, int last, int qexp) {
+  __shared__ float turn[4][32 * 33];
+  const OrthoTile t = w.upd[ortho_id()];
+  const OrthoDesc d = w.desc[t.mat];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nr = ortho_tiles(d.r), nc = ortho_tiles(d.c), nu = (d.c + 255) / 256;
+  const int ti = t.at / nu, tj = t.at % nu * 4 + wave;
+  if (tj >= nc) return;
+  const int64_t now = (k & 1) * d.step, next = d.step - now, tile = (int64_t)nr * 4 * 1024;
+  floatx16 acc[2][2] = {};   // [tile of columns][tile of rows]
+  ortho_product(acc, w.ops + d.xt + now + tj * 2 * tile + lane * 8, w.ops + d.q + ti * 2 * tile + lane * 8, tile, tile, 0,
+                nr * 4);
+  const int32_t* ex = w.exps + t.mat * (ORTHO_MAX_STEPS + 1) + k;
+  const int half = lane >> 5, place = ortho_place(lane & 31);
+  // the sum carries 2^28, Q's and X's scales
+  const float scale = last ? ldexpf(1.f, qexp + ex[0] - 28) : ldexpf(1.f, qexp + ex[0] - ex[1] - 14);
+  float* tt = turn[wave];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int i = i0 + ty + 8 * q, j = j0 + tx;
-    if (i >= d.r || j >= d.c) continue;
-    if (last) ((T*)d.out)[d.flip ? (int64_t)j * d.r + i : (int64_t)i * d.c + j] = from_f<T>(acc[q]);
-    else xn[(int64_t)i * d.c + j] = acc[q];
-  }
+  for (int i = 0; i < 2; ++i)     // rows
+#pragma unroll
+    for (int j = 0; j < 2; ++j) { // columns
+      // this lane: row 32 i + place, columns 32 j + 16 half ..
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = acc[j][i][e] * scale;
+      const bool turned = !last || d.flip;
+      if (turned) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) tt[place * 33 + 16 * half + e] = v[e];
+        wave_lds_sync();
+      }
+      float u[16];                // column 32 j + place, rows 32 i + 16 half ..
+      if (turned) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) u[e] = tt[(16 * half + e) * 33 + place];
+        wave_lds_sync();
+      }
+      if (last) {
+        const int row = ti * 64 + 32 * i, col = tj * 64 + 32 * j;
+        if (d.flip) {
+          if (col + place < d.c)
+            ortho_out<T, 16>((T*)d.out + (int64_t)(col + place) * d.r + row + 16 * half, d.r - row - 16 * half,
+                             d.r % 8 == 0 && (uintptr_t)d.out % 16 == 0, u);
+        } else if (row + place < d.r) {
+          ortho_out<T, 16>((T*)d.out + (int64_t)(row + place) * d.c + col + 16 * half, d.c - col - 16 * half,
+                           d.c % 8 == 0 && (uintptr_t)d.out % 16 == 0, v);
+        }
+      } else {
+        // 16 consecutive k: both halves of one step's fragment
+        half_t* fx = ortho_fragment(w.ops + d.x + next, nc * 4, ti * 2 + i, tj * 4 + j * 2 + half);
+        half_t* ft = ortho_fragment(w.ops + d.xt + next, nr * 4, tj * 2 + j, ti * 4 + i * 2 + half);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          OrthoParts px, pt;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            ortho_split(px, e, v[8 * h + e]);
+            ortho_split(pt, e, u[8 * h + e]);
+          }
+          ortho_put(fx, (lane & 31) + 32 * h, px);
+          ortho_put(ft, (lane & 31) + 32 * h, pt);
+        }
+      }
+    }
 }
 
 struct OrthoPlan {
-  int64_t desc_bytes = 0, parts_bytes = 0, floats = 0;
-  int64_t norm = 0, gram = 0, upd = 0;
-  int64_t bytes() const { return desc_bytes + parts_bytes + 4 * floats; }
+  int64_t halves = 0, parts = 0, gram = 0, upd = 0, count = 0;
+  int64_t o_tiles, o_gram, o_upd, o_parts, o_exps, o_ops, bytes;
 };
 
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Offsets and block counts of every matrix; false: sizes out of range.
+// Offsets and workgroups of every matrix; false: sizes out of range.
 static bool ortho_plan(int count, const lic_ortho_mat* mats, OrthoPlan& p, OrthoDesc* d) {
   for (int i = 0; i < count; ++i) {
     const lic_ortho_mat& m = mats[i];
     if (m.rows < 1 || m.cols < 1 || m.rows > 65536 || m.cols > (1 << 24)) return false;
     const bool flip = m.rows > m.cols;
     const int64_t r = flip ? m.cols : m.rows, c = flip ? m.rows : m.cols;
+    const int64_t nr = up(r, 64) / 64, nc = up(c, 64) / 64, x = nr * nc * 8192, a = nr * nr * 8192;   // halves, both parts
+    if (nr * nc > (1 << 28)) return false;
     OrthoDesc o{m.g, m.out, flip ? m.cs : m.rs, flip ? m.rs : m.cs};
     o.r = (int32_t)r;
     o.c = (int32_t)c;
     o.flip = flip;
-    o.x0 = p.floats;
-    o.x1 = o.x0 + up(r * c, 64);
-    o.a = o.x1 + up(r * c, 64);
-    o.q = o.a + up(r * r, 64);
-    p.floats = o.q + up(r * r, 64);
-    o.norm0 = (int32_t)p.norm;
+    o.step = 2 * x;
+    o.x = p.halves;
+    o.xt = o.x + x;
+    o.a = o.x + 4 * x;
+    o.q = o.a + a;
+    p.halves = o.q + a;
+    o.parts0 = (int32_t)p.parts;
     o.gram0 = (int32_t)p.gram;
     o.upd0 = (int32_t)p.upd;
-    p.norm += (r * c + ORTHO_NORM - 1) / ORTHO_NORM;
-    p.gram += up(r, 32) / 32 * (up(r, 32) / 32);
-    p.upd += up(r, 32) / 32 * (up(c, 32) / 32);
-    if (p.norm > (1 << 30) || p.gram > (1 << 30) || p.upd > (1 << 30)) return false;
+    p.parts += nr * nc;
+    p.gram += nr * (nr + 1) / 2;
+    p.upd += nr * ((nc + 3) / 4);
+    if (p.parts > (1 << 30) || p.gram > (1 << 30) || p.upd > (1 << 30)) return false;
     if (d) d[i] = o;
   }
-  p.desc_bytes = up((int64_t)count * sizeof(OrthoDesc), 256);
-  p.parts_bytes = up(p.norm * 8, 256);
+  p.count += count;
+  p.o_tiles = up(p.count * (int64_t)sizeof(OrthoDesc), 256);
+  p.o_gram = p.o_tiles + up(p.parts * 8, 256);
+  p.o_upd = p.o_gram + up(p.gram * 8, 256);
+  p.o_parts = p.o_upd + up(p.upd * 8, 256);
+  p.o_exps = p.o_parts + up(p.parts * 8, 256);
+  p.o_ops = p.o_exps + up(p.count * 4 * (ORTHO_MAX_STEPS + 1), 256);
+  p.bytes = p.o_ops + 2 * p.halves;
+  return true;
+}
+
+// Bounds of a x + b x^3 + c x^5 on [0, most] and of a + b l + c l^2 on [0, most^2]; false where they run away.
+static bool ortho_bounds(int steps, const float* co, OrthoBounds& o) {
+  const double a = co[0], b = co[1], c = co[2];
+  auto at = [&](double x) { return std::fabs(x * (a + x * x * (b + x * x * c))); };
+  auto q = [&](double l) { return std::fabs(a + l * (b + l * c)); };
+  double most = 1.0, gain = 0.0;
+  o.most[0] = 1.0f;
+  for (int k = 0; k < steps; ++k) {
+    const double l = most * most;
+    double qm = std::fmax(q(0), q(l));
+    if (c != 0 && -b / (2 * c) > 0 && -b / (2 * c) < l) qm = std::fmax(qm, q(-b / (2 * c)));
+    gain = std::fmax(gain, qm);
+    int e;
+    (void)std::frexp(qm * 1.01, &e);
+    o.qexp[k] = qm > 0 ? e : 0;
+    double pm = at(most);
+    // extrema: a + 3 b u + 5 c u^2 = 0, u = x^2
+    const double disc = 9 * b * b - 20 * a * c;
+    double u[2] = {-1, -1};
+    if (c != 0 && disc >= 0) {
+      u[0] = (-3 * b + std::sqrt(disc)) / (10 * c);
+      u[1] = (-3 * b - std::sqrt(disc)) / (10 * c);
+    } else if (c == 0 && b != 0) {
+      u[0] = -a / (3 * b);
+    }
+    for (double v : u)
+      if (v > 0 && v < l) pm = std::fmax(pm, at(std::sqrt(v)));
+    most = pm * 1.01;   // rounding errors on top
+    if (!(most < 1e9)) return false;
+    o.most[k + 1] = (float)most;
+  }
+  o.gain = (float)(gain * 1.01);
   return true;
 }
 
 template <typename T>
-static int ortho_run(const OrthoPlan& p, int count, const lic_ortho_mat* mats, int steps, const float* co, float eps,
-                     char* ws, hipStream_t s) {
-  OrthoDesc* desc = (OrthoDesc*)ws;
-  double* parts = (double*)(ws + p.desc_bytes);
-  float* f = (float*)(ws + p.desc_bytes + p.parts_bytes);
+static int ortho_run(const OrthoPlan& p, int count, const lic_ortho_mat* mats, int steps, const float* co,
+                     const OrthoBounds& bounds, float eps, char* ws, hipStream_t s) {
+  OrthoWork w{(OrthoDesc*)ws, (OrthoTile*)(ws + p.o_tiles), (OrthoTile*)(ws + p.o_gram), (OrthoTile*)(ws + p.o_upd),
+              (double*)(ws + p.o_parts), (int32_t*)(ws + p.o_exps), (half_t*)(ws + p.o_ops)};
   OrthoPlan q;
   OrthoBatch b;
-  // the offsets are those of the whole list: planned again in batches of descriptors
-  for (int i = 0; i < count; i += ORTHO_BATCH) {
-    const int k = count - i < ORTHO_BATCH ? count - i : ORTHO_BATCH;
-    if (!ortho_plan(k, mats + i, q, b.d)) return fail("orthogonalize: sizes out of range");
-    hipLaunchKernelGGL(ortho_desc_kernel, dim3(1), dim3(64), 0, s, b, i, k, desc);
-    LIC_CHECK_LAUNCH();
+  for (int i = 0; i < count; i += ORTHO_BATCH) {   // offsets run on from batch to batch
+    const int n = count - i < ORTHO_BATCH ? count - i : ORTHO_BATCH;
+    if (!ortho_plan(n, mats + i, q, b.d)) return fail("orthogonalize: sizes out of range");
+    hipLaunchKernelGGL(ortho_setup_kernel, dim3(n), dim3(256), 0, s, b, i, w);
   }
-  hipLaunchKernelGGL(ortho_norm_kernel<T>, dim3((unsigned)p.norm), dim3(256), 0, s, desc, count, parts);
-  hipLaunchKernelGGL(ortho_scale_kernel<T>, dim3((unsigned)p.norm), dim3(256), 0, s, desc, count, parts, eps, f);
+  hipLaunchKernelGGL(ortho_norm_kernel<T>, dim3((unsigned)p.parts), dim3(256), 0, s, w);
+  hipLaunchKernelGGL(ortho_scale_kernel<T>, dim3((unsigned)p.parts), dim3(256), 0, s, w, bounds, steps, eps);
   for (int k = 0; k < steps; ++k) {
-    for (int stage = 0; stage < 2; ++stage)
-      hipLaunchKernelGGL(ortho_gram_kernel, dim3((unsigned)p.gram), dim3(256), 0, s, desc, count, f, k & 1, stage, co[0],
-                         co[1], co[2]);
-    hipLaunchKernelGGL(ortho_update_kernel<T>, dim3((unsigned)p.upd), dim3(256), 0, s, desc, count, f, k & 1,
-                       k == steps - 1);
+    hipLaunchKernelGGL(ortho_gram_kernel<0>, dim3((unsigned)p.gram), dim3(512), 0, s, w, k, steps, co[0], co[1], co[2], 0);
+    hipLaunchKernelGGL(ortho_gram_kernel<1>, dim3((unsigned)p.gram), dim3(512), 0, s, w, k, steps, co[0], co[1], co[2],
+                       bounds.qexp[k]);
+    hipLaunchKernelGGL(ortho_update_kernel<T>, dim3((unsigned)p.upd), dim3(256), 0, s, w, k, k == steps - 1,
+                       bounds.qexp[k]);
   }
   LIC_CHECK_LAUNCH();
   return 0;
@@ -204,7 +488,7 @@ extern "C" int64_t lic_orthogonalize_workspace(int32_t dtype, int32_t count, con
   using namespace lic;
   OrthoPlan p;
   if (count < 0 || (count && !mats) || !ortho_plan(count, mats, p, nullptr)) return -1;
-  return p.bytes();
+  return p.bytes;
 }
 
 extern "C" int lic_orthogonalize(int32_t dtype, int32_t count, const lic_ortho_mat* mats, int32_t steps,
@@ -212,16 +496,18 @@ extern "C" int lic_orthogonalize(int32_t dtype, int32_t count, const lic_ortho_m
   using namespace lic;
   if (dtype != LIC_F32 && dtype != LIC_F16 && dtype != LIC_BF16) return fail("orthogonalize: bad dtype");
   if (count < 0 || (count && !mats) || !coeffs) return fail("orthogonalize: null pointer");
-  if (steps < 1 || steps > 64) return fail("orthogonalize: steps out of range");
-  if (!(eps >= 0.f)) return fail("orthogonalize: eps has to be >= 0");
+  if (steps < 1 || steps > ORTHO_MAX_STEPS) return fail("orthogonalize: steps out of range");
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return fail("orthogonalize: eps has to be >= 0");
   if (count == 0) return 0;
   OrthoPlan p;
   if (!ortho_plan(count, mats, p, nullptr)) return fail("orthogonalize: sizes out of range");
   for (int i = 0; i < count; ++i)
     if (!mats[i].g || !mats[i].out) return fail("orthogonalize: null matrix");
-  if (!ws || (uintptr_t)ws % 256 || ws_bytes < p.bytes()) return fail("orthogonalize: workspace missing, misaligned or too small");
+  OrthoBounds bounds;
+  if (!ortho_bounds(steps, coeffs, bounds)) return fail("orthogonalize: the coefficients let the matrices run away");
+  if (!ws || (uintptr_t)ws % 256 || ws_bytes < p.bytes) return fail("orthogonalize: workspace missing, misaligned or too small");
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == LIC_F32) return ortho_run<float>(p, count, mats, steps, coeffs, eps, (char*)ws, s);
-  if (dtype == LIC_F16) return ortho_run<half_t>(p, count, mats, steps, coeffs, eps, (char*)ws, s);
-  return ortho_run<bf16_t>(p, count, mats, steps, coeffs, eps, (char*)ws, s);
+  if (dtype == LIC_F32) return ortho_run<float>(p, count, mats, steps, coeffs, bounds, eps, (char*)ws, s);
+  if (dtype == LIC_F16) return ortho_run<half_t>(p, count, mats, steps, coeffs, bounds, eps, (char*)ws, s);
+  return ortho_run<bf16_t>(p, count, mats, steps, coeffs, bounds, eps, (char*)ws, s);
 }
