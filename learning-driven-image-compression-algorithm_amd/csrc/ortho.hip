@@ -12,7 +12,9 @@
 // lane's 16 results (rows 8 (i / 4) + 4 (lane / 32) + i % 4 of the instruction) are 16 consecutive rows, a whole k step of the
 // transposed operand.  X is kept in both orders: rows along r for A = X X^T, rows along c (X^T) for Q X.
 #include "lic_common.h"
+#include <algorithm>
 #include <cmath>
+#include <vector>
 
 namespace lic {
 
@@ -28,6 +30,8 @@ struct OrthoDesc {
   int32_t r, c, flip;   // flip: out is the transpose of X
   int32_t parts0;       // first of its 64 x 64 tiles' partial sums of |G|^2
   int32_t gram0, upd0;  // first workgroup of A's lower triangle, and of X
+  int32_t slices;       // workgroups that share a tile of A = X X^T
+  int32_t slice0, sum0; // first of them, and of the tiles that are summed up from more than one
 };
 
 // The workgroups of a stage in matrix order.
@@ -39,6 +43,8 @@ struct OrthoBatch { OrthoDesc d[ORTHO_BATCH]; };
 struct OrthoWork {
   OrthoDesc* desc;
   OrthoTile *tiles, *gram, *upd;   // 64 x 64 tiles of G, lower tiles of A, 64 x 256 tiles of X
+  OrthoTile *slices, *sums;        // slices of lower tiles, tiles of several slices
+  float* partial;                  // [slice][4096]
   double* parts;
   int32_t* exps;                   // [count][ORTHO_MAX_STEPS + 1] exponents of X's scale
   half_t* ops;
@@ -59,13 +65,22 @@ __global__ __launch_bounds__(256) void ortho_setup_kernel(OrthoBatch b, int firs
   for (int i = threadIdx.x; i < nr * nc; i += 256) w.tiles[d.parts0 + i] = {mat, i};
   for (int i = threadIdx.x; i < nr * nu; i += 256) w.upd[d.upd0 + i] = {mat, i};
   for (int i = threadIdx.x; i < nr; i += 256)
-    for (int j = 0; j <= i; ++j) w.gram[d.gram0 + i * (i + 1) / 2 + j] = {mat, i << 16 | j};
+    for (int j = 0; j <= i; ++j) {
+      const int at = i * (i + 1) / 2 + j;
+      w.gram[d.gram0 + at] = {mat, i << 16 | j};
+      for (int k = 0; k < d.slices; ++k) w.slices[d.slice0 + at * d.slices + k] = {mat, i << 16 | j};
+      if (d.slices > 1) w.sums[d.sum0 + at] = {mat, i << 16 | j};
+    }
 }
 
-// Workgroups go round the 8 XCDs: a run of neighbouring tiles for each, which share operands in its L2.
+// Workgroups go round the 8 XCDs: ORTHO_RUN neighbouring tiles, which share operands in an L2, for each in turn (longer runs
+// would give one XCD all the tiles of the longest matrices).
+constexpr int ORTHO_RUN = 16;   // codec-sized lists: 432 us; 1: 504, 4: 447, 8: 440
 __device__ __forceinline__ int ortho_id() {
-  const int n = gridDim.x, xcd = blockIdx.x & 7, per = n >> 3, more = n & 7;
-  return xcd * per + min(xcd, more) + (int)(blockIdx.x >> 3);
+  const int b = blockIdx.x, round = 8 * ORTHO_RUN;
+  if (b >= (int)gridDim.x / round * round) return b;
+  const int xcd = b & 7, slot = b >> 3;
+  return slot / ORTHO_RUN * round + xcd * ORTHO_RUN + slot % ORTHO_RUN;
 }
 
 __device__ __forceinline__ int ortho_place(int p) { return (((p >> 2) & 1) << 4) | (((p >> 3) & 3) << 2) | (p & 3); }
@@ -75,7 +90,7 @@ template <typename T, typename F>
 __device__ __forceinline__ void ortho_read(const OrthoDesc& d, int i0, int j0, F f) {
   const bool along = d.cs <= d.rs;   // columns are the nearer ones
   const int fast = threadIdx.x & 63, slow = threadIdx.x >> 6;
-#pragma unroll 4
+#pragma unroll
   for (int s = 0; s < 16; ++s) {
     const int i = along ? slow * 16 + s : fast, j = along ? fast : slow * 16 + s;
     const bool in = i0 + i < d.r && j0 + j < d.c;
@@ -83,7 +98,8 @@ __device__ __forceinline__ void ortho_read(const OrthoDesc& d, int i0, int j0, F
   }
 }
 
-// Sums of squares in 64 bits: the squares of small gradients are below fp32's range.
+// Sums of squares in 64 bits: the squares of small gradients are below fp32's range.  A matrix without gaps is read as a
+// line, 4096 elements a workgroup.
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoWork w) {
   __shared__ double red[4];
@@ -91,7 +107,25 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoWork w) {
   const OrthoDesc d = w.desc[t.mat];
   const int nc = ortho_tiles(d.c);
   double s = 0;
-  ortho_read<T>(d, t.at / nc * 64, t.at % nc * 64, [&](int, int, float v) { s += (double)v * (double)v; });
+  if ((d.cs == 1 && d.rs == d.c) || (d.rs == 1 && d.cs == d.r)) {
+    constexpr int V = 16 / sizeof(T);
+    typedef T Vec __attribute__((ext_vector_type(V)));
+    const T* g = (const T*)d.g;
+    const int64_t total = (int64_t)d.r * d.c, first = (int64_t)t.at * 4096;
+    if ((uintptr_t)g % 16 == 0 && first + 4096 <= total) {
+      Vec v[16 / V];
+#pragma unroll
+      for (int i = 0; i < 16 / V; ++i) v[i] = ((const Vec*)(g + first))[i * 256 + threadIdx.x];
+#pragma unroll
+      for (int i = 0; i < 16 / V; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += (double)to_f(v[i][e]) * (double)to_f(v[i][e]);
+    } else {
+      for (int64_t e = first + threadIdx.x; e < first + 4096 && e < total; e += 256) s += (double)to_f(g[e]) * (double)to_f(g[e]);
+    }
+  } else {
+    ortho_read<T>(d, t.at / nc * 64, t.at % nc * 64, [&](int, int, float v) { s += (double)v * (double)v; });
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -170,8 +204,8 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(OrthoWork w, OrthoBoun
 // 64 x 64 results of P R^T over k steps [s0, s1), operands in fragment order (two row tiles each): acc[i][j] is P's tile i
 // against R's tile j.
 // Steps that the matrix instructions sum up before the rounded fp32 addition to the total: their own additions of a long chain
-// lose more.  2-norm error at 2048 x 2048: one chain 8.9e-6, chains of 16 steps 4.0e-6, of 8 3.3e-6, of 4 3.1e-6 (fp32
-// products: 5.6e-6); 128 x 576: 2.9e-6, .., 2.6e-6 (2.2e-6).  4 costs 1 to 3 % of the time.
+// lose more.  2-norm error at 2048 x 2048: one chain 8.9e-6, chains of 16 steps 4.0e-6, of 8 3.3e-6, of 4 3.0e-6 (fp32
+// products: 5.6e-6); 128 x 576: 2.9e-6, .., 2.4e-6 (2.2e-6).  4 costs 1 to 3 % of the time.
 constexpr int ORTHO_CHAIN = 4;
 struct OrthoFrags { half8 p[2][2], r[2][2]; };
 __device__ __forceinline__ void ortho_load(OrthoFrags& f, const half_t* p, const half_t* r, int64_t ptile, int64_t rtile,
@@ -184,9 +218,10 @@ __device__ __forceinline__ void ortho_load(OrthoFrags& f, const half_t* p, const
       f.r[i][h] = *(const half8*)(r + i * rtile + (int64_t)s * 1024 + h * 512);
     }
 }
+// The small products first, while the sums that they are added to are small.
 __device__ __forceinline__ void ortho_multiply(floatx16 (&acc)[2][2], const OrthoFrags& f) {
 #pragma unroll
-  for (int q = 0; q < 3; ++q)   // hi hi, hi lo, lo hi
+  for (int q = 2; q >= 0; --q)   // lo hi, hi lo, hi hi
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -203,8 +238,10 @@ __device__ __forceinline__ void ortho_product(floatx16 (&sum)[2][2], const half_
     const int end = s + ORTHO_CHAIN < s1 ? s + ORTHO_CHAIN : s1;
     for (; s + 2 <= end; s += 2) {
       ortho_load(f1, p, r, ptile, rtile, s + 1);
+      __builtin_amdgcn_sched_barrier(0);
       ortho_multiply(acc, f0);
       ortho_load(f0, p, r, ptile, rtile, s + 2 < s1 ? s + 2 : s);
+      __builtin_amdgcn_sched_barrier(0);
       ortho_multiply(acc, f1);
     }
     if (s < end) {   // the last step of all
@@ -220,52 +257,18 @@ __device__ __forceinline__ void ortho_product(floatx16 (&sum)[2][2], const half_
   }
 }
 
-// A = X X^T (STAGE 0), or Q = a I + b A + c A A (STAGE 1): a 64 x 64 tile of the lower triangle a workgroup, mirrored.  The 8
-// waves take an eighth of k each and are joined in LDS in a fixed order: a single long matrix has few tiles.
-template <int STAGE>
-__global__ __launch_bounds__(512) void ortho_gram_kernel(OrthoWork w, int k, int steps, float ca, float cb, float cc, int qexp) {
-  __shared__ float join[4][4096];   // [wave][tile of 32 x 32][result][lane]; then the tile, [64][ORTHO_LD]
-  const OrthoTile t = w.gram[ortho_id()];
-  const OrthoDesc d = w.desc[t.mat];
+// A 64 x 64 tile of the lower triangle of A = X X^T (STAGE 0) or Q = a I + b A + c A A (STAGE 1), and its mirror image, from
+// the sums in LDS (which carry 2^28): 8 fragments among the waves.
+template <int STAGE, int NW>
+__device__ __forceinline__ void ortho_lower(const OrthoWork& w, const OrthoDesc& d, int mat, int at, const float* out, int k,
+                                            float ca, float cb, float cc, int qexp) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int ti = t.at >> 16, tj = t.at & 0xffff, nr = ortho_tiles(d.r), nc = ortho_tiles(d.c);
-  const half_t* op = w.ops + (STAGE == 0 ? d.x + (k & 1) * d.step : d.a);
-  const int ksteps = (STAGE == 0 ? nc : nr) * 4;
-  const int64_t tile = (int64_t)ksteps * 1024;
-  floatx16 acc[2][2] = {};
-  ortho_product(acc, op + ti * 2 * tile + lane * 8, op + tj * 2 * tile + lane * 8, tile, tile, ksteps * wave / 8,
-                ksteps * (wave + 1) / 8);
-  if (wave >= 4) {
+  const int ti = at >> 16, tj = at & 0xffff, nr = ortho_tiles(d.r);
 #pragma unroll
-    for (int e = 0; e < 64; ++e) join[wave - 4][e * 64 + lane] = acc[e >> 5][(e >> 4) & 1][e & 15];
-  }
-  __syncthreads();
-  if (wave < 4) {
-#pragma unroll
-    for (int e = 0; e < 64; ++e) join[wave][e * 64 + lane] += acc[e >> 5][(e >> 4) & 1][e & 15];
-  }
-  __syncthreads();
-  float v[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int at = e * 512 + threadIdx.x;
-    v[e] = (join[0][at] + join[1][at]) + (join[2][at] + join[3][at]);
-  }
-  __syncthreads();
-  float* out = &join[0][0];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int at = e * 512 + threadIdx.x, l = at & 63, f = at >> 6, i = f & 15, b = (f >> 4) & 1, a = f >> 5;
-    out[(32 * a + 16 * (l >> 5) + i) * ORTHO_LD + 32 * b + ortho_place(l & 31)] = v[e];
-  }
-  __syncthreads();
-  // a fragment a wave, and the mirrored tile's
-  const int rt = wave >> 2, ks = wave & 3;
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
+  for (int g = 0; g < 16 / NW; ++g) {
+    const int m = g / (8 / NW), f8 = g % (8 / NW) * NW + wave, rt = f8 >> 2, ks = f8 & 3;
     if (m == 1 && ti == tj) break;
     const int I = m ? tj : ti, J = m ? ti : tj;
-    // the sum carries 2^28
     OrthoParts p;
     if constexpr (STAGE == 0) {
       p = m ? ortho_gather<true>(out, rt, ks, lane, 0x1p-14f) : ortho_gather<false>(out, rt, ks, lane, 0x1p-14f);
@@ -273,7 +276,7 @@ __global__ __launch_bounds__(512) void ortho_gram_kernel(OrthoWork w, int k, int
     } else {
       const half_t* f = ortho_fragment(w.ops + d.a, nr * 4, I * 2 + rt, J * 4 + ks);
       const half8 hi = *(const half8*)(f + lane * 8), lo = *(const half8*)(f + 512 + lane * 8);
-      const int e2 = 2 * w.exps[t.mat * (ORTHO_MAX_STEPS + 1) + k];
+      const int e2 = 2 * w.exps[mat * (ORTHO_MAX_STEPS + 1) + k];
       const float s1 = ldexpf(cb, e2 - 14), s2 = ldexpf(cc, 2 * e2 - 28), down = ldexpf(1.f, 14 - qexp);
       const int row = 32 * rt + ortho_place(lane & 31), col = 16 * ks + 8 * (lane >> 5);
 #pragma unroll
@@ -286,6 +289,78 @@ __global__ __launch_bounds__(512) void ortho_gram_kernel(OrthoWork w, int k, int
       ortho_put(ortho_fragment(w.ops + d.q, nr * 4, I * 2 + rt, J * 4 + ks), lane, p);
     }
   }
+}
+
+// A thread's sums of a tile (place e * 64 NW + thread of the joined order) to LDS, [64][ORTHO_LD].
+template <int NW>
+__device__ __forceinline__ void ortho_spread(float* out, const float* v) {
+#pragma unroll
+  for (int e = 0; e < 64 / NW; ++e) {
+    const int at = e * 64 * NW + threadIdx.x, l = at & 63, f = at >> 6, i = f & 15, b = (f >> 4) & 1, a = f >> 5;
+    out[(32 * a + 16 * (l >> 5) + i) * ORTHO_LD + 32 * b + ortho_place(l & 31)] = v[e];
+  }
+}
+
+// A tile of the lower triangle a workgroup.  Its NW waves take a part of k each and are joined in LDS in a fixed order: a
+// single long matrix has few tiles.  STAGE 0: of a slice of k where there are several; their sums go on to
+// ortho_sum_kernel.
+template <int STAGE, int NW>
+__global__ __launch_bounds__(64 * NW) void ortho_gram_kernel(OrthoWork w, int k, float ca, float cb, float cc, int qexp) {
+  __shared__ float join[NW / 2 < 2 ? 2 : NW / 2][4096];   // [wave][tile of 32 x 32][result][lane]; then the tile, [64][ORTHO_LD]
+  const int id = ortho_id();
+  const OrthoTile t = STAGE == 0 ? w.slices[id] : w.gram[id];
+  const OrthoDesc d = w.desc[t.mat];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ti = t.at >> 16, tj = t.at & 0xffff, nr = ortho_tiles(d.r), nc = ortho_tiles(d.c);
+  const half_t* op = w.ops + (STAGE == 0 ? d.x + (k & 1) * d.step : d.a);
+  const int ksteps = (STAGE == 0 ? nc : nr) * 4;
+  const int64_t tile = (int64_t)ksteps * 1024;
+  const int shares = STAGE == 0 ? NW * d.slices : NW, share = STAGE == 0 ? (id - d.slice0) % d.slices * NW + wave : wave;
+  floatx16 acc[2][2] = {};
+  ortho_product(acc, op + ti * 2 * tile + lane * 8, op + tj * 2 * tile + lane * 8, tile, tile,
+                (int)((int64_t)ksteps * share / shares), (int)((int64_t)ksteps * (share + 1) / shares));
+  if (wave >= NW / 2) {
+#pragma unroll
+    for (int e = 0; e < 64; ++e) join[wave - NW / 2][e * 64 + lane] = acc[e >> 5][(e >> 4) & 1][e & 15];
+  }
+  __syncthreads();
+  if (wave < NW / 2) {
+#pragma unroll
+    for (int e = 0; e < 64; ++e) join[wave][e * 64 + lane] += acc[e >> 5][(e >> 4) & 1][e & 15];
+  }
+  __syncthreads();
+  float v[64 / NW];
+#pragma unroll
+  for (int e = 0; e < 64 / NW; ++e) {
+    const int at = e * 64 * NW + threadIdx.x;
+    v[e] = join[0][at] + join[1][at];
+    if constexpr (NW == 8) v[e] += join[2][at] + join[3][at];
+  }
+  if (STAGE == 0 && d.slices > 1) {
+    float* to = w.partial + (int64_t)id * 4096;
+#pragma unroll
+    for (int e = 0; e < 64 / NW; ++e) to[e * 64 * NW + threadIdx.x] = v[e];
+    return;
+  }
+  __syncthreads();
+  ortho_spread<NW>(&join[0][0], v);
+  __syncthreads();
+  ortho_lower<STAGE, NW>(w, d, t.mat, t.at, &join[0][0], k, ca, cb, cc, qexp);
+}
+
+// A from the slices' sums, in their order.
+__global__ __launch_bounds__(512) void ortho_sum_kernel(OrthoWork w) {
+  __shared__ float out[64 * ORTHO_LD];
+  const OrthoTile t = w.sums[blockIdx.x];
+  const OrthoDesc d = w.desc[t.mat];
+  const float* from = w.partial + (d.slice0 + (int64_t)((int)blockIdx.x - d.sum0) * d.slices) * 4096;
+  float v[8] = {};
+  for (int s = 0; s < d.slices; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += from[s * 4096 + e * 512 + threadIdx.x];
+  ortho_spread<8>(out, v);
+  __syncthreads();
+  ortho_lower<0, 8>(w, d, t.mat, t.at, out, 0, 0.f, 0.f, 0.f, 0);
 }
 
 template <typename T, int N>
@@ -316,7 +391,9 @@ __global__ __launch_bounds__(256) void ortho_update_kernel(OrthoWork w, int k, i
   const OrthoDesc d = w.desc[t.mat];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nr = ortho_tiles(d.r), nc = ortho_tiles(d.c), nu = (d.c + 255) / 256;
-  const int ti = t.at / nu, tj = t.at % nu * 4 + wave;
+  // workgroups of one group of columns follow each other (in groups of 8 tiles of rows): they share X's fragments in the L2
+  const int group = t.at / (8 * nu), rest = t.at - group * 8 * nu, rows = min(8, nr - group * 8);
+  const int ti = group * 8 + rest % rows, tj = rest / rows * 4 + wave;
   if (tj >= nc) return;
   const int64_t now = (k & 1) * d.step, next = d.step - now, tile = (int64_t)nr * 4 * 1024;
   floatx16 acc[2][2] = {};   // [tile of columns][tile of rows]
@@ -377,9 +454,15 @@ __global__ __launch_bounds__(256) void ortho_update_kernel(OrthoWork w, int k, i
 }
 
 struct OrthoPlan {
-  int64_t halves = 0, parts = 0, gram = 0, upd = 0, count = 0;
-  int64_t o_tiles, o_gram, o_upd, o_parts, o_exps, o_ops, bytes;
+  int64_t halves = 0, parts = 0, gram = 0, upd = 0, slices = 0, partials = 0, sums = 0, count = 0;
+  int64_t o_tiles, o_gram, o_upd, o_slices, o_sums, o_parts, o_exps, o_partial, o_ops, bytes;
 };
+
+// A tile's k is shared out among workgroups in slices of at least ORTHO_SLICE steps of 16 while a matrix has fewer than
+// ORTHO_FILL of them (192 x 4800: 259 -> 169 us, 192 x 1728: 164 -> 149; with 16 steps 183, 149).  From ORTHO_MANY
+// workgroups on they have 4 waves, two of them on a compute unit, instead of 8 (2048 x 2048: 840 -> 790 us; 128 x 576, of 3:
+// 114 -> 119).
+constexpr int ORTHO_SLICE = 32, ORTHO_FILL = 256, ORTHO_MANY = 512;
 
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -405,19 +488,32 @@ static bool ortho_plan(int count, const lic_ortho_mat* mats, OrthoPlan& p, Ortho
     o.parts0 = (int32_t)p.parts;
     o.gram0 = (int32_t)p.gram;
     o.upd0 = (int32_t)p.upd;
+    // slices of k of at least ORTHO_SLICE steps where the tiles of A are few
+    const int64_t lower = nr * (nr + 1) / 2, most = ORTHO_FILL / lower;
+    o.slices = (int32_t)std::max<int64_t>(1, std::min(nc * 4 / ORTHO_SLICE, most));
+    o.slice0 = (int32_t)p.slices;
+    o.sum0 = (int32_t)p.sums;
+    p.slices += lower * o.slices;
+    if (o.slices > 1) {
+      p.sums += lower;
+      p.partials = p.slices;
+    }
     p.parts += nr * nc;
-    p.gram += nr * (nr + 1) / 2;
+    p.gram += lower;
     p.upd += nr * ((nc + 3) / 4);
-    if (p.parts > (1 << 30) || p.gram > (1 << 30) || p.upd > (1 << 30)) return false;
+    if (p.parts > (1 << 30) || p.slices > (1 << 30) || p.upd > (1 << 30)) return false;
     if (d) d[i] = o;
   }
   p.count += count;
   p.o_tiles = up(p.count * (int64_t)sizeof(OrthoDesc), 256);
   p.o_gram = p.o_tiles + up(p.parts * 8, 256);
   p.o_upd = p.o_gram + up(p.gram * 8, 256);
-  p.o_parts = p.o_upd + up(p.upd * 8, 256);
+  p.o_slices = p.o_upd + up(p.upd * 8, 256);
+  p.o_sums = p.o_slices + up(p.slices * 8, 256);
+  p.o_parts = p.o_sums + up(p.sums * 8, 256);
   p.o_exps = p.o_parts + up(p.parts * 8, 256);
-  p.o_ops = p.o_exps + up(p.count * 4 * (ORTHO_MAX_STEPS + 1), 256);
+  p.o_partial = p.o_exps + up(p.count * 4 * (ORTHO_MAX_STEPS + 1), 256);
+  p.o_ops = p.o_partial + p.partials * 4096 * 4;
   p.bytes = p.o_ops + 2 * p.halves;
   return true;
 }
@@ -461,9 +557,13 @@ template <typename T>
 static int ortho_run(const OrthoPlan& p, int count, const lic_ortho_mat* mats, int steps, const float* co,
                      const OrthoBounds& bounds, float eps, char* ws, hipStream_t s) {
   OrthoWork w{(OrthoDesc*)ws, (OrthoTile*)(ws + p.o_tiles), (OrthoTile*)(ws + p.o_gram), (OrthoTile*)(ws + p.o_upd),
-              (double*)(ws + p.o_parts), (int32_t*)(ws + p.o_exps), (half_t*)(ws + p.o_ops)};
+              (OrthoTile*)(ws + p.o_slices), (OrthoTile*)(ws + p.o_sums), (float*)(ws + p.o_partial), (double*)(ws + p.o_parts), (int32_t*)(ws + p.o_exps), (half_t*)(ws + p.o_ops)};
   OrthoPlan q;
   OrthoBatch b;
+  std::vector<lic_ortho_mat> sorted(mats, mats + count);   // the longest products start first
+  auto shorter = [](const lic_ortho_mat& m) { return std::min(m.rows, m.cols); };
+  std::stable_sort(sorted.begin(), sorted.end(), [&](const lic_ortho_mat& x, const lic_ortho_mat& y) { return shorter(x) > shorter(y); });
+  mats = sorted.data();
   for (int i = 0; i < count; i += ORTHO_BATCH) {   // offsets run on from batch to batch
     const int n = count - i < ORTHO_BATCH ? count - i : ORTHO_BATCH;
     if (!ortho_plan(n, mats + i, q, b.d)) return fail("orthogonalize: sizes out of range");
@@ -472,9 +572,17 @@ static int ortho_run(const OrthoPlan& p, int count, const lic_ortho_mat* mats, i
   hipLaunchKernelGGL(ortho_norm_kernel<T>, dim3((unsigned)p.parts), dim3(256), 0, s, w);
   hipLaunchKernelGGL(ortho_scale_kernel<T>, dim3((unsigned)p.parts), dim3(256), 0, s, w, bounds, steps, eps);
   for (int k = 0; k < steps; ++k) {
-    hipLaunchKernelGGL(ortho_gram_kernel<0>, dim3((unsigned)p.gram), dim3(512), 0, s, w, k, steps, co[0], co[1], co[2], 0);
-    hipLaunchKernelGGL(ortho_gram_kernel<1>, dim3((unsigned)p.gram), dim3(512), 0, s, w, k, steps, co[0], co[1], co[2],
-                       bounds.qexp[k]);
+    if (p.slices >= ORTHO_MANY)
+      hipLaunchKernelGGL((ortho_gram_kernel<0, 4>), dim3((unsigned)p.slices), dim3(256), 0, s, w, k, 0.f, 0.f, 0.f, 0);
+    else
+      hipLaunchKernelGGL((ortho_gram_kernel<0, 8>), dim3((unsigned)p.slices), dim3(512), 0, s, w, k, 0.f, 0.f, 0.f, 0);
+    if (p.sums) hipLaunchKernelGGL(ortho_sum_kernel, dim3((unsigned)p.sums), dim3(512), 0, s, w);
+    if (p.gram >= ORTHO_MANY)
+      hipLaunchKernelGGL((ortho_gram_kernel<1, 4>), dim3((unsigned)p.gram), dim3(256), 0, s, w, k, co[0], co[1], co[2],
+                         bounds.qexp[k]);
+    else
+      hipLaunchKernelGGL((ortho_gram_kernel<1, 8>), dim3((unsigned)p.gram), dim3(512), 0, s, w, k, co[0], co[1], co[2],
+                         bounds.qexp[k]);
     hipLaunchKernelGGL(ortho_update_kernel<T>, dim3((unsigned)p.upd), dim3(256), 0, s, w, k, k == steps - 1,
                        bounds.qexp[k]);
   }
