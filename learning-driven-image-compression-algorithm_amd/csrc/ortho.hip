@@ -85,6 +85,9 @@ __device__ __forceinline__ int ortho_id() {
 
 __device__ __forceinline__ int ortho_place(int p) { return (((p >> 2) & 1) << 4) | (((p >> 3) & 3) << 2) | (p & 3); }
 
+// G and the result come as addresses from a table: said to be global, so that their accesses are not flat ones.
+template <typename T> using OrthoGlobal = __attribute__((address_space(1))) T*;
+
 // A 64 x 64 tile of G, element (i, j) of it to thread (of 256) and slot (of 16) so that either order of G reads in lines.
 template <typename T, typename F>
 __device__ __forceinline__ void ortho_read(const OrthoDesc& d, int i0, int j0, F f) {
@@ -94,7 +97,7 @@ __device__ __forceinline__ void ortho_read(const OrthoDesc& d, int i0, int j0, F
   for (int s = 0; s < 16; ++s) {
     const int i = along ? slow * 16 + s : fast, j = along ? fast : slow * 16 + s;
     const bool in = i0 + i < d.r && j0 + j < d.c;
-    f(i, j, in ? to_f(((const T*)d.g)[(i0 + i) * d.rs + (j0 + j) * d.cs]) : 0.f);
+    f(i, j, in ? to_f(((OrthoGlobal<const T>)d.g)[(i0 + i) * d.rs + (j0 + j) * d.cs]) : 0.f);
   }
 }
 
@@ -110,12 +113,12 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoWork w) {
   if ((d.cs == 1 && d.rs == d.c) || (d.rs == 1 && d.cs == d.r)) {
     constexpr int V = 16 / sizeof(T);
     typedef T Vec __attribute__((ext_vector_type(V)));
-    const T* g = (const T*)d.g;
+    const OrthoGlobal<const T> g = (OrthoGlobal<const T>)d.g;
     const int64_t total = (int64_t)d.r * d.c, first = (int64_t)t.at * 4096;
-    if ((uintptr_t)g % 16 == 0 && first + 4096 <= total) {
+    if ((uintptr_t)d.g % 16 == 0 && first + 4096 <= total) {
       Vec v[16 / V];
 #pragma unroll
-      for (int i = 0; i < 16 / V; ++i) v[i] = ((const Vec*)(g + first))[i * 256 + threadIdx.x];
+      for (int i = 0; i < 16 / V; ++i) v[i] = ((OrthoGlobal<const Vec>)(g + first))[i * 256 + threadIdx.x];
 #pragma unroll
       for (int i = 0; i < 16 / V; ++i)
 #pragma unroll
@@ -218,7 +221,8 @@ __device__ __forceinline__ void ortho_load(OrthoFrags& f, const half_t* p, const
       f.r[i][h] = *(const half8*)(r + i * rtile + (int64_t)s * 1024 + h * 512);
     }
 }
-// The small products first, while the sums that they are added to are small.
+// The small products first, while the sums that they are added to are small.  FIRST: of a chain, which starts from zero.
+template <bool FIRST>
 __device__ __forceinline__ void ortho_multiply(floatx16 (&acc)[2][2], const OrthoFrags& f) {
 #pragma unroll
   for (int q = 2; q >= 0; --q)   // lo hi, hi lo, hi hi
@@ -226,34 +230,48 @@ __device__ __forceinline__ void ortho_multiply(floatx16 (&acc)[2][2], const Orth
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.p[i][q == 2], f.r[j][q == 1], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.p[i][q == 2], f.r[j][q == 1],
+                                                           FIRST && q == 2 ? floatx16{} : acc[i][j], 0, 0, 0);
+}
+__device__ __forceinline__ void ortho_sum(floatx16 (&sum)[2][2], const floatx16 (&acc)[2][2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum[i][j][e] += acc[i][j][e];
 }
 __device__ __forceinline__ void ortho_product(floatx16 (&sum)[2][2], const half_t* p, const half_t* r, int64_t ptile,
                                               int64_t rtile, int s0, int s1) {
   if (s0 >= s1) return;
   OrthoFrags f0, f1;   // one step is multiplied while the next one is under way
-  ortho_load(f0, p, r, ptile, rtile, s0);
-  for (int s = s0; s < s1;) {
-    floatx16 acc[2][2] = {};
-    const int end = s + ORTHO_CHAIN < s1 ? s + ORTHO_CHAIN : s1;
-    for (; s + 2 <= end; s += 2) {
-      ortho_load(f1, p, r, ptile, rtile, s + 1);
-      __builtin_amdgcn_sched_barrier(0);
-      ortho_multiply(acc, f0);
-      ortho_load(f0, p, r, ptile, rtile, s + 2 < s1 ? s + 2 : s);
-      __builtin_amdgcn_sched_barrier(0);
-      ortho_multiply(acc, f1);
+  floatx16 acc[2][2];
+  auto load = [&](OrthoFrags& f, int s) {
+    ortho_load(f, p, r, ptile, rtile, s < s1 ? s : s1 - 1);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  load(f0, s0);
+  int s = s0;
+  for (; s + ORTHO_CHAIN <= s1; s += ORTHO_CHAIN) {
+#pragma unroll
+    for (int c = 0; c < ORTHO_CHAIN; c += 2) {
+      load(f1, s + c + 1);
+      if (c == 0) ortho_multiply<true>(acc, f0);
+      else ortho_multiply<false>(acc, f0);
+      load(f0, s + c + 2);
+      ortho_multiply<false>(acc, f1);
     }
-    if (s < end) {   // the last step of all
-      ortho_multiply(acc, f0);
-      ++s;
+    ortho_sum(sum, acc);
+  }
+  if (s < s1) {   // up to three steps
+    load(f1, s + 1);
+    ortho_multiply<true>(acc, f0);
+    if (s + 1 < s1) {
+      load(f0, s + 2);
+      ortho_multiply<false>(acc, f1);
+      if (s + 2 < s1) ortho_multiply<false>(acc, f0);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sum[i][j][e] += acc[i][j][e];
+    ortho_sum(sum, acc);
   }
 }
 
@@ -305,7 +323,7 @@ __device__ __forceinline__ void ortho_spread(float* out, const float* v) {
 // single long matrix has few tiles.  STAGE 0: of a slice of k where there are several; their sums go on to
 // ortho_sum_kernel.
 template <int STAGE, int NW>
-__global__ __launch_bounds__(64 * NW) void ortho_gram_kernel(OrthoWork w, int k, float ca, float cb, float cc, int qexp) {
+__global__ __launch_bounds__(64 * NW, 2) void ortho_gram_kernel(OrthoWork w, int k, float ca, float cb, float cc, int qexp) {
   __shared__ float join[NW / 2 < 2 ? 2 : NW / 2][4096];   // [wave][tile of 32 x 32][result][lane]; then the tile, [64][ORTHO_LD]
   const int id = ortho_id();
   const OrthoTile t = STAGE == 0 ? w.slices[id] : w.gram[id];
@@ -364,7 +382,7 @@ __global__ __launch_bounds__(512) void ortho_sum_kernel(OrthoWork w) {
 }
 
 template <typename T, int N>
-__device__ __forceinline__ void ortho_out(T* out, int count, bool wide, const float* v) {
+__device__ __forceinline__ void ortho_out(OrthoGlobal<T> out, int count, bool wide, const float* v) {
   if (wide && count >= N) {
     constexpr int E = 16 / sizeof(T);
     typedef T Vec __attribute__((ext_vector_type(E)));
@@ -373,7 +391,7 @@ __device__ __forceinline__ void ortho_out(T* out, int count, bool wide, const fl
       Vec o;
 #pragma unroll
       for (int f = 0; f < E; ++f) o[f] = from_f<T>(v[e + f]);
-      *(Vec*)(out + e) = o;
+      *(OrthoGlobal<Vec>)(out + e) = o;
     }
   } else {
 #pragma unroll
@@ -385,7 +403,7 @@ __device__ __forceinline__ void ortho_out(T* out, int count, bool wide, const fl
 // X <- Q X: 64 rows x 64 columns a wave, 64 x 256 a workgroup (Q's fragments are shared through the L1).  The last step
 // writes the result instead.
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_update_kernel(OrthoWork w, int k, int last, int qexp) {
+__global__ __launch_bounds__(256, 2) void ortho_update_kernel(OrthoWork w, int k, int last, int qexp) {
   __shared__ float turn[4][32 * 33];
   const OrthoTile t = w.upd[ortho_id()];
   const OrthoDesc d = w.desc[t.mat];
@@ -428,10 +446,10 @@ __global__ __launch_bounds__(256) void ortho_update_kernel(OrthoWork w, int k, i
         const int row = ti * 64 + 32 * i, col = tj * 64 + 32 * j;
         if (d.flip) {
           if (col + place < d.c)
-            ortho_out<T, 16>((T*)d.out + (int64_t)(col + place) * d.r + row + 16 * half, d.r - row - 16 * half,
+            ortho_out<T, 16>((OrthoGlobal<T>)d.out + (int64_t)(col + place) * d.r + row + 16 * half, d.r - row - 16 * half,
                              d.r % 8 == 0 && (uintptr_t)d.out % 16 == 0, u);
         } else if (row + place < d.r) {
-          ortho_out<T, 16>((T*)d.out + (int64_t)(row + place) * d.c + col + 16 * half, d.c - col - 16 * half,
+          ortho_out<T, 16>((OrthoGlobal<T>)d.out + (int64_t)(row + place) * d.c + col + 16 * half, d.c - col - 16 * half,
                            d.c % 8 == 0 && (uintptr_t)d.out % 16 == 0, v);
         }
       } else {
