@@ -15,7 +15,7 @@
  *    (data, n, h, w, c, ld): `data` already points at the first channel of the
  *    view, `ld` is the element stride between consecutive pixels, so channel
  *    slices / concatenations (torch.cat, torch.split, chunk) are free.
- *  - dtype tag: LIC_F32 or LIC_F16 for activations and packed weights; biases,
+ *  - dtype tag: LIC_F32, LIC_F16 or LIC_BF16 for activations and packed weights; biases,
  *    GDN/LayerNorm parameters, scales and metrics are always fp32.
  *  - All tensors are caller-owned device memory; the library never allocates,
  *    frees or retains.  Calls are asynchronous on the given stream and are safe
@@ -599,7 +599,8 @@ int lic_wba16_qkv_attn_fwd(const lic_wba16_args* a, lic_stream_t stream);
  * table: device, per pair {uint64 freq / 2pi in units of 2^-64 turns (mod 1), int32 axis, int32 0}.
  * pos: int32 [naxes][n][h*w] (pos_per_image != 0) or [naxes][h*w], contiguous; NULL: the grid's own
  * positions, naxes 1: y*w + x, 2: (y, x), 3: (image, y, x).  y == x (same ld) rotates in place; other
- * overlaps are the caller's to avoid.  naxes <= LIC_ROTARY_MAX_AXES. */
+ * overlaps are the caller's to avoid.  naxes <= LIC_ROTARY_MAX_AXES; up to 2^31 tokens, 8192 channels a
+ * head, 2^18 channels a token. */
 #define LIC_ROTARY_MAX_AXES 4
 enum lic_rotary_layout { LIC_ROTARY_HALF = 0, LIC_ROTARY_PAIRS = 1 };
 int lic_rotary(int32_t dtype, const void* x, int32_t ldx, int32_t n, int32_t h, int32_t w, int32_t c,
@@ -610,13 +611,13 @@ int lic_rotary(int32_t dtype, const void* x, int32_t ldx, int32_t n, int32_t h, 
 /* Products in 8-bit integers with a scale for each token (row of x) and output channel.
  * lic_quantize_int8: codes[i][j] = rint(127 x[i][j] / max_j |x[i][j]|) (exact, half to even; zero for a
  * zero row), scale[i] = max_j |x[i][j]| / 127, columns [k, kpad) zero; a row that holds a NaN or an infinity
- * gets zero codes and a NaN scale, which makes its whole output row NaN.  Also packs weights (rows =
- * output channels).  kpad: a multiple of 64, >= k; codes 16-byte aligned.
+ * gets zero codes and a NaN scale, which makes its whole result NaN (a ReLU, v > 0 ? v : 0, ends it as
+ * elsewhere in this library).  Also packs weights (rows = output channels).  kpad: a multiple of 64, >= k; codes 16-byte aligned.
  * lic_linear_int8: y[i][o] = act(xscale[i] * wscale[o] * sum_j xcodes[i][j] * w[o][j] + bias[o]) + r1[i][o],
  * the sum in 32-bit integers (k <= 131072 cannot overflow), the rest in fp32, rounded once to `dtype`.
  * Either xcodes / xscale ([m][kpad], fp32 [m]) or x (m rows of k, stride ldx, quantised by the call) is given.
  * act: LIC_ACT_NONE / RELU / LRELU / GELU; bias and r1 may be NULL; y must not overlap x, xcodes or w (r1 may
- * be y).  ws: lic_linear_int8_workspace bytes, 16-byte aligned (needed with x only; 0 with xcodes). */
+ * be y).  ws: with x, lic_linear_int8_workspace bytes, 16-byte aligned (0: up to 4 tokens of kpad <= 4096). */
 #define LIC_INT8_MAX_K 131072
 int lic_quantize_int8(int32_t dtype, const void* x, int64_t ldx, int32_t m, int32_t k, int8_t* codes, int32_t kpad,
                       float* scale, lic_stream_t stream);
@@ -629,7 +630,10 @@ int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const int8_t* xco
 /* Newton-Schulz orthogonalisation of `count` matrices at once (the update of the Muon optimiser):
  *   X = G / (|G|_F + eps);  `steps` times: A = X X^T, X = (a I + b A + c A A) X     (on G^T if rows > cols)
  * g: `dtype` elements at g + i*rs + j*cs (any strides), out: rows x cols, contiguous, `dtype`.  `mats` is a
- * host array (read before the call returns).  coeffs = {a, b, c}.  Deterministic (no atomics).
+ * host array (read before the call returns).  coeffs = {a, b, c}; refused where they let |X| grow beyond
+ * 1e9.  Products of two fp16 parts each (22 bits), fp32 sums: the error of fp32 products.  A zero matrix
+ * gives zeros, one with a NaN or an infinity nothing finite.  Deterministic (no atomics); a matrix's result
+ * does not depend on its neighbours in the list.
  * ws: lic_orthogonalize_workspace bytes of device memory, 256-byte aligned, -1: sizes out of range. */
 typedef struct lic_ortho_mat {
   const void* g; int64_t rs, cs;

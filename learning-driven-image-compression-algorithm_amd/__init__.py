@@ -3,7 +3,7 @@ learned image codec of xiaobucc/learning-driven-image-compression-algorithm.
 
 Layout mirrors the reference: ``layers/`` (GDN, window attention,
 Win_noShift_Attention, compressai blocks), ``model/`` (net_ga, net_unet_ha_hs,
-Block_unet, gdn), ``ops/`` (LowerBound, NonNegativeParametrizer).  Every
+Block_unet, gdn), ``ops/`` (LowerBound, NonNegativeParametrizer); ``optim`` has the Muon optimiser.  Every
 activation-sized op runs in liblic.so (csrc/, C ABI in include/lic.h) through
 ``_ffi`` (ctypes); ``functional`` holds the tensor-level wrappers.
 """

@@ -445,12 +445,12 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
   int8_join<T, TT>(a, part, acc, n0, m0, a.xs);
 }
 
-// One to ONE_TOKENS tokens in one launch: every workgroup quantises them into LDS, its first weights already under way.
-constexpr int ONE_TOKENS = 4, ONE_VECS = 2;   // a thread's part of a row: ONE_VECS loads of 16 bytes
-template <typename T> constexpr int one_max_k() { return 512 * ONE_VECS * 16 / (int)sizeof(T); }
-template <typename T>
+// One to ONE_TOKENS tokens of up to ONE_K channels in one launch: every workgroup quantises them into LDS, its first weights
+// already under way.
+constexpr int ONE_TOKENS = 4, ONE_K = 4096;
+template <typename T, int V>
 __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int VECS = ONE_K / 512 / V;   // a thread's part of a row
   typedef QuantVec<T, V> Vec;
   __shared__ int part[8][1][256];
   __shared__ uint32_t most[ONE_TOKENS][8];
@@ -465,13 +465,13 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
 #pragma unroll
   for (int u = 0; u < 8; ++u)
     if (s0 + u < s1) fw[u] = *(const int32x4*)(w + 64 * (s0 + u));
-  Vec v[ONE_TOKENS][ONE_VECS];
+  Vec v[ONE_TOKENS][VECS];
 #pragma unroll
   for (int r = 0; r < ONE_TOKENS; ++r) {
     if (r >= a.m) break;
     QuantMax<T> top;
 #pragma unroll
-    for (int i = 0; i < ONE_VECS; ++i) {
+    for (int i = 0; i < VECS; ++i) {
       const int j = (threadIdx.x + 512 * i) * V;
       v[r][i] = Vec{};
       if (j < a.k) v[r][i] = *(const Vec*)((const T*)a.x + r * a.ldx + j);
@@ -496,16 +496,20 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
     if (threadIdx.x == 0) scale[r] = top / 127.f;
     const QuantRow qr = quant_row(top);
 #pragma unroll
-    for (int i = 0; i < ONE_VECS; ++i) {
+    for (int i = 0; i < VECS; ++i) {
       const int j = (threadIdx.x + 512 * i) * V;
       if (j < a.kpad) {
         float f[V];
-        uint32_t c[V / 4] = {};
+        uint32_t c[(V + 3) / 4] = {};
 #pragma unroll
         for (int e = 0; e < V; ++e) f[e] = to_f(v[r][i][e]);
         if (qr.inv != 0.f) quant_codes<T, V>(f, qr, c);
+        if constexpr (V == 1) {
+          codes[r * a.kpad + j] = (int8_t)c[0];
+        } else {
 #pragma unroll
-        for (int e = 0; e < V / 4; ++e) ((uint32_t*)(codes + r * a.kpad + j))[e] = c[e];
+          for (int e = 0; e < V / 4; ++e) ((uint32_t*)(codes + r * a.kpad + j))[e] = c[e];
+        }
       }
     }
   }
@@ -729,9 +733,9 @@ static int few_launch(const Int8Args& a, hipStream_t s) {
   return 0;
 }
 
-template <typename T>
+template <typename T, int V>
 static int one_launch(const Int8Args& a, hipStream_t s) {
-  hipLaunchKernelGGL(int8_one_kernel<T>, dim3((a.n + 15) / 16), dim3(512), a.m * a.kpad, s, a);
+  hipLaunchKernelGGL((int8_one_kernel<T, V>), dim3((a.n + 15) / 16), dim3(512), a.m * a.kpad, s, a);
   LIC_CHECK_LAUNCH();
   return 0;
 }
@@ -743,7 +747,7 @@ static int linear_run(Int8Args a, int8_t* codes, float* scale, hipStream_t s) {
   a.wide = a.act != LIC_ACT_GELU && p % 16 == 0 && a.ldy % E == 0 && (!a.r1 || a.ldr1 % E == 0);
   if (a.x) {
     const bool aligned = (uintptr_t)a.x % 16 == 0 && a.ldx % E == 0 && a.k % E == 0;
-    if (aligned && a.m <= ONE_TOKENS && a.kpad <= one_max_k<T>()) return one_launch<T>(a, s);
+    if (a.m <= ONE_TOKENS && a.kpad <= ONE_K) return aligned ? one_launch<T, 16 / sizeof(T)>(a, s) : one_launch<T, 1>(a, s);
     // us, 192 -> 576 fp16 (quantised apart, tiles): 131072 tokens 54.4 (97), 16384: 16.0 (20.1), 8192: 13.4 (14.5), 4096: 12
     // (10); 384 -> 384: 79.5 (94); from kpad 448 on the operands spill; fp32, 192 -> 576: 32768 tokens 34 (45), 8192: 21 (17.5)
     if (aligned && a.m >= (sizeof(T) == 2 ? 8192 : 16384) && a.kpad <= 384 && a.wide && a.n % 32 == 0) return rows_run<T>(a, s);
@@ -781,6 +785,7 @@ extern "C" int lic_quantize_int8(int32_t dtype, const void* x, int64_t ldx, int3
 
 extern "C" int64_t lic_linear_int8_workspace(int32_t m, int32_t kpad) {
   if (m < 0 || kpad < 1 || kpad > LIC_INT8_MAX_K) return -1;
+  if (m <= lic::ONE_TOKENS && kpad <= lic::ONE_K) return 0;   // quantised in LDS
   const int64_t codes = (int64_t)m * kpad;
   return (codes + 15) / 16 * 16 + 4 * (int64_t)m;
 }
@@ -800,8 +805,8 @@ extern "C" int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const 
   hipStream_t s = (hipStream_t)stream;
   if (x) {
     if (ldx < k) return fail("linear_int8: row stride below k");
-    if (!ws || (uintptr_t)ws % 16 || ws_bytes < lic_linear_int8_workspace(m, kpad))
-      return fail("linear_int8: workspace missing, misaligned or too small");
+    const int64_t need = lic_linear_int8_workspace(m, kpad);
+    if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need)) return fail("linear_int8: workspace missing, misaligned or too small");
   }
   Int8Args a{xcodes, xscale, w, wscale, bias, r1, y, x, ldr1, ldy, ldx, m, n, k, kpad, act, slope, 0};
   int8_t* codes = (int8_t*)ws;

@@ -1067,12 +1067,16 @@ def recon(xtil: Act, wgen: Act, mode: int, post: Optional[torch.Tensor] = None, 
 # --------------------------------------------------------------------------- rotary positions
 def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """The launch goes to the current device's current stream: operands of another device are refused."""
+    dev = -1
     for t in tensors:
-        if t is not None and not t.is_cuda:
+        if t is None:
+            continue
+        at = t.get_device()
+        if at < 0:
             raise ValueError(f"{what}: tensor is not on the GPU (move the module / inputs to 'cuda')")
-    dev = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != dev:
+        if dev < 0:
+            dev = torch.cuda.current_device()
+        if at != dev:
             raise ValueError(f"{what}: tensor on {t.device}, the current device is cuda:{dev}")
 
 
@@ -1265,7 +1269,8 @@ def linear_int8(x, pk: Int8Pack, out: Optional[Act] = None, *, act: int = _ffi.A
     m, kpad = B * H * W, pk.w.shape[1]
     if m == 0:
         return out
-    nbytes = 0 if q is not None else -(-m * kpad // 16) * 16 + 4 * m      # lic_linear_int8_workspace
+    # lic_linear_int8_workspace
+    nbytes = 0 if q is not None or (m <= 4 and kpad <= 4096) else -(-m * kpad // 16) * 16 + 4 * m
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=src.device) if nbytes else None
     r1p, ldr1 = _ptr(r1)
     check(_lib().lic_linear_int8(dtype_id(dtype), None if q is not None else x.ptr, 0 if q is not None else x.ld,

@@ -54,6 +54,16 @@ class Muon(torch.optim.Optimizer):
     def _scale(adjust: str, rows: int, cols: int) -> float:
         return 0.2 * math.sqrt(max(rows, cols)) if adjust == "rms" else math.sqrt(max(1.0, rows / cols))
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # the base class casts floating state to the parameter's dtype: the momentum stays fp32
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(ids, params):
+            saved = state_dict["state"].get(i, {})
+            if "momentum" in saved:
+                self.state[p]["momentum"] = saved["momentum"].detach().to(device=p.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

@@ -203,3 +203,18 @@ def test_muon_captured_step_matches_eager():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(eager, cap))
+
+
+@pytest.mark.parametrize("mode", ["--eager", "--graph"])
+def test_train_cli_with_muon(mode, monkeypatch, capsys):
+    """train_net_unet.py --optimizer muon (at its 256 x 256 crops, which the net's windows need): eager and captured steps
+    run and print a finite epoch summary."""
+    import re
+    import sys
+    import train_net_unet
+    monkeypatch.setattr(sys, "argv", ["train_net_unet.py", "--optimizer", "muon", mode, "--batch_size", "1",
+                                      "--steps_per_epoch", "2", "--warmup", "2", "--lr", "1e-4"])
+    train_net_unet.main()
+    out = capsys.readouterr().out
+    loss = float(re.search(r"\[Epoch 0000 TRAIN\] Loss: (\S+)", out).group(1))
+    assert math.isfinite(loss) and loss > 0

@@ -143,10 +143,12 @@ def test_c_entry_refusals():
     _refused(lin(x=None, xc=f), "x or xcodes")
     _refused(lin(w=f + 4), "aligned")
     _refused(lin(ldx=99), "stride below k")
-    _refused(lin(work=None), "workspace")
-    _refused(lin(nbytes=16), "workspace")
+    _refused(lin(m=5, work=None), "workspace")
+    _refused(lin(m=5, work=f + 8), "workspace")
+    _refused(lin(m=5, nbytes=16), "workspace")
     assert lin(m=0) == 0
-    assert lib.lic_linear_int8_workspace(4, 128) > 4 * 128 and lib.lic_linear_int8_workspace(-1, 128) == -1
+    assert lib.lic_linear_int8_workspace(5, 128) >= 5 * 128 + 20 and lib.lic_linear_int8_workspace(-1, 128) == -1
+    assert lib.lic_linear_int8_workspace(4, 4096) == 0 and lib.lic_linear_int8_workspace(4, 4160) > 0
 
     def ortho(rows=8, cols=8, g=f, out=f, steps=5, eps=1e-7, dtype=0, count=1, ws=f, nbytes=1 << 30, coeffs=True):
         m = (_ffi.OrthoMat * 1)()
@@ -167,6 +169,11 @@ def test_c_entry_refusals():
     _refused(ortho(ws=f + 8), "workspace")
     _refused(ortho(nbytes=64), "workspace")
     assert ortho(count=0) == 0
+    m = (_ffi.OrthoMat * 1)()
+    m[0].g, m[0].rs, m[0].cs, m[0].out, m[0].rows, m[0].cols = f, 8, 1, f, 8, 8
+    wild = (ctypes.c_float * 3)(10.0, 10.0, 10.0)
+    _refused(lib.lic_orthogonalize(0, 1, m, 9, wild, 1e-7, f, 1 << 30, None), "run away")
+    assert lib.lic_orthogonalize_workspace(0, 1, m) > 0 and lib.lic_orthogonalize_workspace(0, -1, m) == -1
 
 
 def test_ortho_struct_matches_c_compiler(tmp_path):
@@ -203,6 +210,17 @@ def test_muon_refusals_and_split():
         Muon(mats, momentum=1.0)
     with pytest.raises(ValueError, match="lr"):
         Muon(mats, lr=-1.0)
+
+
+def test_muon_state_keeps_fp32_momentum():
+    from lic_amd.optim import Muon
+    p = torch.nn.Parameter(torch.zeros(8, 8, dtype=torch.bfloat16))
+    a, b = Muon([p]), Muon([p])
+    a.state[p]["momentum"] = torch.randn(8, 8) * 1.2345678
+    b.load_state_dict(a.state_dict())
+    got = b.state[p]["momentum"]
+    assert got.dtype == torch.float32 and torch.equal(got, a.state[p]["momentum"])
+    assert got.data_ptr() != a.state[p]["momentum"].data_ptr()
 
 
 def test_int8_context_is_nested_and_thread_local():
