@@ -32,6 +32,7 @@ struct OrthoDesc {
   int32_t gram0, upd0;  // first workgroup of A's lower triangle, and of X
   int32_t slices;       // workgroups that share a tile of A = X X^T
   int32_t slice0, sum0; // first of them, and of the tiles that are summed up from more than one
+  int32_t partial0;     // first of the slices' sums
 };
 
 // The workgroups of a stage in matrix order.
@@ -44,7 +45,7 @@ struct OrthoWork {
   OrthoDesc* desc;
   OrthoTile *tiles, *gram, *upd;   // 64 x 64 tiles of G, lower tiles of A, 64 x 256 tiles of X
   OrthoTile *slices, *sums;        // slices of lower tiles, tiles of several slices
-  float* partial;                  // [slice][4096]
+  float* partial;                  // [slice of a tile that has several][4096]
   double* parts;
   int32_t* exps;                   // [count][ORTHO_MAX_STEPS + 1] exponents of X's scale
   half_t* ops;
@@ -277,14 +278,14 @@ __device__ __forceinline__ void ortho_product(floatx16 (&sum)[2][2], const half_
 
 // A 64 x 64 tile of the lower triangle of A = X X^T (STAGE 0) or Q = a I + b A + c A A (STAGE 1), and its mirror image, from
 // the sums in LDS (which carry 2^28): 8 fragments among the waves.
-template <int STAGE, int NW>
+template <int STAGE>
 __device__ __forceinline__ void ortho_lower(const OrthoWork& w, const OrthoDesc& d, int mat, int at, const float* out, int k,
                                             float ca, float cb, float cc, int qexp) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ti = at >> 16, tj = at & 0xffff, nr = ortho_tiles(d.r);
 #pragma unroll
-  for (int g = 0; g < 16 / NW; ++g) {
-    const int m = g / (8 / NW), f8 = g % (8 / NW) * NW + wave, rt = f8 >> 2, ks = f8 & 3;
+  for (int g = 0; g < 4; ++g) {
+    const int m = g / 2, f8 = g % 2 * 4 + wave, rt = f8 >> 2, ks = f8 & 3;
     if (m == 1 && ti == tj) break;
     const int I = m ? tj : ti, J = m ? ti : tj;
     OrthoParts p;
@@ -309,22 +310,21 @@ __device__ __forceinline__ void ortho_lower(const OrthoWork& w, const OrthoDesc&
   }
 }
 
-// A thread's sums of a tile (place e * 64 NW + thread of the joined order) to LDS, [64][ORTHO_LD].
-template <int NW>
+// A thread's sums of a tile (place e * 256 + thread of the joined order) to LDS, [64][ORTHO_LD].
 __device__ __forceinline__ void ortho_spread(float* out, const float* v) {
 #pragma unroll
-  for (int e = 0; e < 64 / NW; ++e) {
-    const int at = e * 64 * NW + threadIdx.x, l = at & 63, f = at >> 6, i = f & 15, b = (f >> 4) & 1, a = f >> 5;
+  for (int e = 0; e < 16; ++e) {
+    const int at = e * 256 + threadIdx.x, l = at & 63, f = at >> 6, i = f & 15, b = (f >> 4) & 1, a = f >> 5;
     out[(32 * a + 16 * (l >> 5) + i) * ORTHO_LD + 32 * b + ortho_place(l & 31)] = v[e];
   }
 }
 
-// A tile of the lower triangle a workgroup.  Its NW waves take a part of k each and are joined in LDS in a fixed order: a
-// single long matrix has few tiles.  STAGE 0: of a slice of k where there are several; their sums go on to
+// A tile of the lower triangle a workgroup.  Its four waves take a quarter of k each and are joined in LDS in a fixed order:
+// a single long matrix has few tiles.  STAGE 0: of a slice of k where there are several; their sums go on to
 // ortho_sum_kernel.
-template <int STAGE, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void ortho_gram_kernel(OrthoWork w, int k, float ca, float cb, float cc, int qexp) {
-  __shared__ float join[NW / 2 < 2 ? 2 : NW / 2][4096];   // [wave][tile of 32 x 32][result][lane]; then the tile, [64][ORTHO_LD]
+template <int STAGE>
+__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(OrthoWork w, int k, float ca, float cb, float cc, int qexp) {
+  __shared__ float join[2][4096];   // [wave][tile of 32 x 32][result][lane]; then the tile, [64][ORTHO_LD]
   const int id = ortho_id();
   const OrthoTile t = STAGE == 0 ? w.slices[id] : w.gram[id];
   const OrthoDesc d = w.desc[t.mat];
@@ -333,52 +333,49 @@ __global__ __launch_bounds__(64 * NW, 2) void ortho_gram_kernel(OrthoWork w, int
   const half_t* op = w.ops + (STAGE == 0 ? d.x + (k & 1) * d.step : d.a);
   const int ksteps = (STAGE == 0 ? nc : nr) * 4;
   const int64_t tile = (int64_t)ksteps * 1024;
-  const int shares = STAGE == 0 ? NW * d.slices : NW, share = STAGE == 0 ? (id - d.slice0) % d.slices * NW + wave : wave;
+  const int shares = STAGE == 0 ? 4 * d.slices : 4, share = STAGE == 0 ? (id - d.slice0) % d.slices * 4 + wave : wave;
   floatx16 acc[2][2] = {};
   ortho_product(acc, op + ti * 2 * tile + lane * 8, op + tj * 2 * tile + lane * 8, tile, tile,
                 (int)((int64_t)ksteps * share / shares), (int)((int64_t)ksteps * (share + 1) / shares));
-  if (wave >= NW / 2) {
+  if (wave >= 2) {
 #pragma unroll
-    for (int e = 0; e < 64; ++e) join[wave - NW / 2][e * 64 + lane] = acc[e >> 5][(e >> 4) & 1][e & 15];
+    for (int e = 0; e < 64; ++e) join[wave - 2][e * 64 + lane] = acc[e >> 5][(e >> 4) & 1][e & 15];
   }
   __syncthreads();
-  if (wave < NW / 2) {
+  if (wave < 2) {
 #pragma unroll
     for (int e = 0; e < 64; ++e) join[wave][e * 64 + lane] += acc[e >> 5][(e >> 4) & 1][e & 15];
   }
   __syncthreads();
-  float v[64 / NW];
+  float v[16];
 #pragma unroll
-  for (int e = 0; e < 64 / NW; ++e) {
-    const int at = e * 64 * NW + threadIdx.x;
-    v[e] = join[0][at] + join[1][at];
-    if constexpr (NW == 8) v[e] += join[2][at] + join[3][at];
-  }
+  for (int e = 0; e < 16; ++e) v[e] = join[0][e * 256 + threadIdx.x] + join[1][e * 256 + threadIdx.x];
   if (STAGE == 0 && d.slices > 1) {
-    float* to = w.partial + (int64_t)id * 4096;
+    float* part = w.partial + (int64_t)(id - d.slice0 + d.partial0) * 4096;
 #pragma unroll
-    for (int e = 0; e < 64 / NW; ++e) to[e * 64 * NW + threadIdx.x] = v[e];
+    for (int e = 0; e < 16; ++e) part[e * 256 + threadIdx.x] = v[e];
     return;
   }
   __syncthreads();
-  ortho_spread<NW>(&join[0][0], v);
+  ortho_spread(&join[0][0], v);
   __syncthreads();
-  ortho_lower<STAGE, NW>(w, d, t.mat, t.at, &join[0][0], k, ca, cb, cc, qexp);
+  ortho_lower<STAGE>(w, d, t.mat, t.at, &join[0][0], k, ca, cb, cc, qexp);
 }
 
 // A from the slices' sums, in their order.
-__global__ __launch_bounds__(512) void ortho_sum_kernel(OrthoWork w) {
+__global__ __launch_bounds__(256) void ortho_sum_kernel(OrthoWork w) {
   __shared__ float out[64 * ORTHO_LD];
   const OrthoTile t = w.sums[blockIdx.x];
   const OrthoDesc d = w.desc[t.mat];
-  const float* from = w.partial + (d.slice0 + (int64_t)((int)blockIdx.x - d.sum0) * d.slices) * 4096;
-  float v[8] = {};
+  const float* from = w.partial + (d.partial0 + (int64_t)((int)blockIdx.x - d.sum0) * d.slices) * 4096;
+  float v[16] = {};
+#pragma unroll 3   // 192 x 4800: 167.6 -> 161.8 us
   for (int s = 0; s < d.slices; ++s)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += from[s * 4096 + e * 512 + threadIdx.x];
-  ortho_spread<8>(out, v);
+    for (int e = 0; e < 16; ++e) v[e] += from[s * 4096 + e * 256 + threadIdx.x];
+  ortho_spread(out, v);
   __syncthreads();
-  ortho_lower<0, 8>(w, d, t.mat, t.at, out, 0, 0.f, 0.f, 0.f, 0);
+  ortho_lower<0>(w, d, t.mat, t.at, out, 0, 0.f, 0.f, 0.f, 0);
 }
 
 template <typename T, int N>
@@ -477,14 +474,14 @@ struct OrthoPlan {
 };
 
 // A tile's k is shared out among workgroups in slices of at least ORTHO_SLICE steps of 16 while a matrix has fewer than
-// ORTHO_FILL of them (192 x 4800: 259 -> 169 us, 192 x 1728: 164 -> 149; with 16 steps 183, 149).  From ORTHO_MANY
-// workgroups on they have 4 waves, two of them on a compute unit, instead of 8 (2048 x 2048: 840 -> 790 us; 128 x 576, of 3:
-// 114 -> 119).
-constexpr int ORTHO_SLICE = 32, ORTHO_FILL = 256, ORTHO_MANY = 512;
+// ORTHO_FILL of them (one slice / 20 / 32 steps: 192 x 4800: 259 / 172 / 165 us; the codec's list 428 / 439 / 410).  Both
+// are rules of the matrix alone, and so is the four waves' part: its result is the same in any list (eight waves:
+// 128 x 576 108.6 us, with four 110.8; 2048 x 2048 810 us, with four 739).
+constexpr int ORTHO_SLICE = 32, ORTHO_FILL = 256;
 
 static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Offsets and workgroups of every matrix; false: sizes out of range.
+// Offsets and workgroups of every matrix (the totals do not depend on the matrices' order); false: sizes out of range.
 static bool ortho_plan(int count, const lic_ortho_mat* mats, OrthoPlan& p, OrthoDesc* d) {
   for (int i = 0; i < count; ++i) {
     const lic_ortho_mat& m = mats[i];
@@ -511,10 +508,11 @@ static bool ortho_plan(int count, const lic_ortho_mat* mats, OrthoPlan& p, Ortho
     o.slices = (int32_t)std::max<int64_t>(1, std::min(nc * 4 / ORTHO_SLICE, most));
     o.slice0 = (int32_t)p.slices;
     o.sum0 = (int32_t)p.sums;
+    o.partial0 = (int32_t)p.partials;
     p.slices += lower * o.slices;
     if (o.slices > 1) {
       p.sums += lower;
-      p.partials = p.slices;
+      p.partials += lower * o.slices;
     }
     p.parts += nr * nc;
     p.gram += lower;
@@ -590,17 +588,10 @@ static int ortho_run(const OrthoPlan& p, int count, const lic_ortho_mat* mats, i
   hipLaunchKernelGGL(ortho_norm_kernel<T>, dim3((unsigned)p.parts), dim3(256), 0, s, w);
   hipLaunchKernelGGL(ortho_scale_kernel<T>, dim3((unsigned)p.parts), dim3(256), 0, s, w, bounds, steps, eps);
   for (int k = 0; k < steps; ++k) {
-    if (p.slices >= ORTHO_MANY)
-      hipLaunchKernelGGL((ortho_gram_kernel<0, 4>), dim3((unsigned)p.slices), dim3(256), 0, s, w, k, 0.f, 0.f, 0.f, 0);
-    else
-      hipLaunchKernelGGL((ortho_gram_kernel<0, 8>), dim3((unsigned)p.slices), dim3(512), 0, s, w, k, 0.f, 0.f, 0.f, 0);
-    if (p.sums) hipLaunchKernelGGL(ortho_sum_kernel, dim3((unsigned)p.sums), dim3(512), 0, s, w);
-    if (p.gram >= ORTHO_MANY)
-      hipLaunchKernelGGL((ortho_gram_kernel<1, 4>), dim3((unsigned)p.gram), dim3(256), 0, s, w, k, co[0], co[1], co[2],
-                         bounds.qexp[k]);
-    else
-      hipLaunchKernelGGL((ortho_gram_kernel<1, 8>), dim3((unsigned)p.gram), dim3(512), 0, s, w, k, co[0], co[1], co[2],
-                         bounds.qexp[k]);
+    hipLaunchKernelGGL(ortho_gram_kernel<0>, dim3((unsigned)p.slices), dim3(256), 0, s, w, k, 0.f, 0.f, 0.f, 0);
+    if (p.sums) hipLaunchKernelGGL(ortho_sum_kernel, dim3((unsigned)p.sums), dim3(256), 0, s, w);
+    hipLaunchKernelGGL(ortho_gram_kernel<1>, dim3((unsigned)p.gram), dim3(256), 0, s, w, k, co[0], co[1], co[2],
+                       bounds.qexp[k]);
     hipLaunchKernelGGL(ortho_update_kernel<T>, dim3((unsigned)p.upd), dim3(256), 0, s, w, k, k == steps - 1,
                        bounds.qexp[k]);
   }

@@ -112,6 +112,19 @@ def test_orthogonalize_many_and_eps():
         _check(o, a, eps=0.0)
 
 
+def test_orthogonalize_result_does_not_depend_on_the_list():
+    """Long lists, whose many tiles take kernels of another shape, give every matrix the bits that it has alone."""
+    import lic_amd.functional as Fn
+    g = torch.Generator().manual_seed(8)
+    shapes = [(192, 1728)] * 12 + [(256, 2304)] * 4 + [(300, 300), (40, 5000), (128, 576), (700, 800), (2048, 2048)]
+    mats = [_gradient(m, n, g, torch.float32).to(DEV) for m, n in shapes]
+    outs = Fn.orthogonalize(mats)
+    for a, o in zip(mats, outs):
+        assert torch.equal(Fn.orthogonalize([a])[0], o), tuple(a.shape)
+    for a, o in zip(mats[:1] + mats[-3:], outs[:1] + outs[-3:]):
+        _check(o, a)
+
+
 def test_orthogonalize_streams_and_graph():
     import lic_amd.functional as Fn
     lists = [[torch.randn(96, 160, device=DEV), torch.randn(200, 64, device=DEV)], [torch.randn(128, 128, device=DEV)]]
