@@ -112,6 +112,91 @@ def test_linear_int8_matches_64_bits(dtype, m, k, n):
     assert torch.equal(Fn.linear_int8(Fn.quantize_tokens(xa), pk).t, got)
 
 
+# whole rows in one launch (many tokens of few aligned channels; fp32 from 16384 tokens on) and the large tiles (with one to
+# five steps of k, whole and ragged columns)
+LARGE = [(16384, 64, 64), (16401, 128, 32), (16390, 192, 576), (16399, 200, 96), (16384, 256, 160), (16500, 320, 64),
+         (16389, 384, 384), (16384, 8, 32), (2048, 40, 2048), (2050, 100, 2050), (2100, 190, 2047), (2048, 300, 2080),
+         (4096, 40, 4096), (4103, 100, 4100), (4096, 190, 4097), (4100, 300, 4096)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", LARGE)
+def test_linear_int8_large(dtype, m, k, n):
+    import lic_amd.functional as Fn
+    g = torch.Generator(device=DEV).manual_seed(m + 7 * k + 13 * n)
+    x = (torch.randn(m, k, generator=g, device=DEV) * 3).to(dtype)
+    x[7], x[9, 3] = 0, float("nan")
+    w, b = torch.randn(n, k, generator=g, device=DEV), torch.randn(n, generator=g, device=DEV)
+    r1 = torch.randn(m, n, generator=g, device=DEV).to(dtype)
+    pk = Fn.pack_linear_int8(w, b)
+    finite = torch.ones(m, dtype=torch.bool, device=DEV)
+    finite[9] = False
+    codes, scale = _codes(x[finite])
+    wc, ws = _codes(w)
+
+    def check(got, act, r):
+        assert torch.isnan(got[9]).all()
+        want, tol = _result(codes, scale, wc, ws, b.double(), act, 0.2, None if r is None else r[finite].double())
+        dt = got.dtype
+        tol = tol * 1.2 + want.abs() * torch.finfo(dt).eps / 2 + (2.0 ** -25 if dt == torch.float16 else 1e-37)
+        assert ((got[finite].double() - want).abs() <= tol).all()
+    xa = Fn.Act(x.view(1, 1, m, k))
+    got = Fn.linear_int8(xa, pk).t
+    check(got.view(m, n), 0, None)
+    assert torch.equal(Fn.linear_int8(Fn.quantize_tokens(xa), pk).t.nan_to_num(), got.nan_to_num())
+    act = (0, 2, 3)[(m + n) % 3]   # not a ReLU, which ends a NaN
+    y = Fn.linear_int8(xa, pk, act=act, slope=0.2, r1=Fn.Act(r1.view(1, 1, m, n))).t
+    check(y.view(m, n), act, r1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_int8_rows_views(dtype):
+    """The launch that takes whole rows, on channel windows (also out = r1): the bits of the quantised map's product,
+    what lies beside and behind the windows left as it was, and a token's bits the same as alone."""
+    import lic_amd.functional as Fn
+    g = torch.Generator(device=DEV).manual_seed(4)
+    m, c, n = 16401, 192, 96
+    x = torch.randn(1, 1, m, c + 32, generator=g, device=DEV).to(dtype)
+    r = torch.randn(1, 1, m, n + 24, generator=g, device=DEV).to(dtype)
+    for bias in (None, torch.randn(n, generator=g, device=DEV)):
+        pk = Fn.pack_linear_int8(torch.randn(n, c, generator=g, device=DEV), bias)
+        xa, ra = Fn.Act(x, 16, c), Fn.Act(r, 8, n)
+        want = Fn.linear_int8(Fn.quantize_tokens(xa), pk, r1=ra, act=2, slope=0.1).t
+        buf = torch.full((1, 2, m, n + 16), 9.0, dtype=dtype, device=DEV)
+        Fn.linear_int8(xa, pk, Fn.Act(buf[:, :1], 8, n), r1=ra, act=2, slope=0.1)
+        assert torch.equal(buf[:, :1, :, 8:8 + n], want)
+        buf[:, :1, :, 8:8 + n] = 9.0
+        assert (buf == 9.0).all()
+        own = r.clone()
+        view = Fn.Act(own, 8, n)
+        Fn.linear_int8(xa, pk, view, r1=view, act=2, slope=0.1)
+        assert torch.equal(own[..., 8:8 + n], want)
+        own[..., 8:8 + n] = r[..., 8:8 + n]
+        assert torch.equal(own, r)
+        for a, b in ((0, 1), (100, 103), (300, 340), (16000, 16401)):
+            part = Fn.linear_int8(Fn.Act(x[:, :, a:b, 16:16 + c].contiguous()), pk, act=2, slope=0.1,
+                                  r1=Fn.Act(r[:, :, a:b, 8:8 + n].contiguous())).t
+            assert torch.equal(part, want[:, :, a:b])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_int8_few_tokens_any_alignment(dtype):
+    """One to six tokens, aligned or not, up to and beyond the channels that one launch quantises: the same bits as
+    quantised beforehand."""
+    import lic_amd.functional as Fn
+    g = torch.Generator(device=DEV).manual_seed(5)
+    for k in (1, 100, 512, 4095, 4096, 4100, 9000):
+        pk = Fn.pack_linear_int8(torch.randn(40, k, generator=g, device=DEV), torch.randn(40, generator=g, device=DEV))
+        x = torch.randn(1, 1, 6, k + 9, generator=g, device=DEV).to(dtype)
+        for m in (1, 2, 3, 4, 5, 6):
+            for c0 in (0, 1, 8):
+                xa = Fn.Act(x[:, :, :m], c0, k)
+                codes, _ = _codes(xa.t[0, 0, :, c0:c0 + k])
+                q = Fn.quantize_tokens(xa)
+                assert torch.equal(q.codes.view(m, -1)[:, :k].double(), codes)
+                assert torch.equal(Fn.linear_int8(xa, pk).t, Fn.linear_int8(q, pk).t), (k, m, c0)
+
+
 def test_linear_int8_rows_do_not_depend_on_the_batch():
     """Integer sums: a token's result is the same bits alone and in any batch, in every form the sizes select."""
     import lic_amd.functional as Fn
