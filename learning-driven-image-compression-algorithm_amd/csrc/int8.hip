@@ -1,4 +1,7 @@
-// Products in 8-bit integers with a scale for each token and output channel (gfx950).
+// Products in 8-bit integers with a scale for each token and output channel (gfx950):
+//   y = act(xs[i] ws[o] sum_j X[i][j] W[o][j] + bias[o]) + r1,  X[i][j] = rint(127 x[i][j] / max_j |x[i][j]|), xs = max / 127.
+// The sum is an integer of 32 bits (exact, so no form or order of it shows in a result), the rest is fp32 and is rounded
+// once, to y's type.  The codes' 8 bits are the operator's definition.
 #include "lic_common.h"
 
 namespace lic {
@@ -105,7 +108,8 @@ template <> struct QuantMax<float> {
 };
 
 // G lanes a row, V elements a load; a lane keeps its part of the row in registers (NV vectors of it; longer rows are read
-// a second time).  Bound by the bytes of x and codes.
+// a second time).  Bound by the bytes of x and codes: 8192 x 4096 bf16 21.5 us, 4.7 TB/s; 1037 x 333 fp32, whose
+// columns allow single elements only, 3.7 us.
 template <typename T, int V, int G>
 __global__ __launch_bounds__(256) void quantize_int8_kernel(const T* __restrict__ x, int64_t ldx, int m, int k,
                                                             int8_t* __restrict__ codes, int kpad,
@@ -278,7 +282,9 @@ __device__ __forceinline__ int int8_channel(int r) {
 
 // Tiled product: BM tokens x BN channels a workgroup of WM x WN waves, 64 bytes of k a step, four steps of both operands
 // in LDS, three of them in flight by LDS-DMA while one is multiplied (one barrier a step).  A row's four 16-byte chunks sit
-// at chunk ^ (row / 2) % 4: eight neighbouring lanes of a fragment read cover all 64 banks.
+// at chunk ^ (row / 2) % 4: eight neighbouring lanes of a fragment read cover all 64 banks.  Bound by the matrix
+// instructions: 8192 x 4096 -> 8192 282 us, 1.95 POP/s (a large library product reaches 2.06); small ones by the latency of
+// their k steps: 128 x 4096 -> 4096 13.1 us, 1037 x 333 -> 517 fp32 8.9 us.
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int mt, int nt) {
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, BK = 64, STAGES = 4;
@@ -406,7 +412,7 @@ __device__ __forceinline__ void int8_join(const Int8Args& a, int (*part)[TT][256
 }
 
 // Few tokens: 16 channels x 16 TT tokens a workgroup, its 8 waves on an eighth of k each, fragments straight from memory.
-// Bound by the weights' bytes, or by latency.
+// Bound by the weights' bytes, or by latency: 16 x 4096 -> 4096 6.5 us (2.6 TB/s), 16 x 192 -> 576 5.4 us.
 template <typename T, int TT>
 __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
   __shared__ int part[8][TT][256];
@@ -446,7 +452,7 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
 }
 
 // One to ONE_TOKENS tokens of up to ONE_K channels in one launch: every workgroup quantises them into LDS, its first weights
-// already under way.
+// already under way.  Bound by latency, then the weights' bytes: 1 x 4096 -> 4096 7.5 us (quantised apart: 5.6 + 5.4).
 constexpr int ONE_TOKENS = 4, ONE_K = 4096;
 template <typename T, int V>
 __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
@@ -526,17 +532,21 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
   int8_join<T, 1>(a, part, acc, n0, 0, scale);
 }
 
-// Many tokens of few channels (kpad = 64 KS; whole tiles of y only: n a multiple of 32, a.wide): 32 tokens a wave, quantised straight into matrix operands that stay in
-// registers; the weights pass through LDS, 64 channels at a time, the next under way.  x is read once and y written once, the
-// codes never reach memory.  A weight row's 16-byte chunks are placed so that a fragment read meets every bank once: rows
-// advance by 16 KS of the 64 words, so chunk ^ swizzle(row) within 4, 8 or 16 chunks spreads those that coincide.
+// Many tokens of few channels (kpad = 64 KS; whole tiles of y only: n a multiple of 32, a.wide): 32 tokens a wave, quantised
+// straight into matrix operands that stay in registers; the weights pass through LDS, 64 channels at a time, the next under
+// way.  x is read once and y written once, the codes never reach memory.  Bound by the bytes of y: 131072 x 192 -> 576 fp16
+// 44 us alone, 53 with the call (201 MB; 35 without its stores).  A weight row's 16-byte chunks are placed so that a fragment
+// read meets every bank once: rows advance by 16 KS of the 64 words, so chunk ^ swizzle(row) within 4, 8 or 16 chunks spreads
+// those that coincide.
 template <int KS>
 __device__ __forceinline__ int int8_rows_swizzle(int r) {
   return KS % 4 == 0 ? r & 15 : KS % 2 == 0 ? (r >> 1) & 7 : (r >> 2) & 3;
 }
 
+// waves a SIMD that the registers and the LDS of a form allow
+template <typename T, int KS> constexpr int ROWS_WAVES = sizeof(T) == 2 ? (KS <= 3 ? 4 : 3) : (KS == 1 ? 4 : KS <= 3 ? 3 : 2);
 template <typename T, int KS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? (KS <= 3 ? 4 : 3) : (KS == 1 ? 4 : KS <= 3 ? 3 : 2)) void int8_rows_kernel(Int8Args a) {
+__global__ __launch_bounds__(256, (ROWS_WAVES<T, KS>)) void int8_rows_kernel(Int8Args a) {
   constexpr int CK = 2 * KS, KP = 64 * KS, V = 16 / sizeof(T), L = 16 / V;   // products of 32 k; loads of 16 elements
   constexpr bool HOLD = CK * 16 * sizeof(T) <= 256;                          // a lane's half row fits 64 registers
   typedef QuantVec<T, V> Vec;
@@ -664,7 +674,7 @@ template <typename T, int KS>
 static int rows_launch(const Int8Args& a, hipStream_t s) {
   // channels are shared out where the token blocks alone would not fill the chip (each share quantises its tokens again)
   const int blocks = (int)(((int64_t)a.m + 127) / 128), chunks = (a.n + 63) / 64;
-  const int shares = blocks >= ROWS_FILL ? 1 : (ROWS_FILL + blocks - 1) / blocks < chunks ? (ROWS_FILL + blocks - 1) / blocks : chunks;
+  const int fill = (ROWS_FILL + blocks - 1) / blocks, shares = fill < chunks ? fill : chunks;
   hipLaunchKernelGGL((int8_rows_kernel<T, KS>), dim3((unsigned)blocks, (unsigned)shares), dim3(256), 0, s, a);
   LIC_CHECK_LAUNCH();
   return 0;
@@ -688,9 +698,13 @@ static void quantize_launch(const void* x, int64_t ldx, int m, int k, int8_t* co
                             hipStream_t s) {
   const int vecs = kpad / V;
   // lanes of a row: up to four vectors each, a whole wave from there on
-  if (vecs <= 32) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 8>), dim3((m + 31) / 32), dim3(256), 0, s, (const T*)x, ldx, m, k, codes, kpad, scale);
-  else if (vecs <= 64) hipLaunchKernelGGL((quantize_int8_kernel<T, V, 16>), dim3((m + 15) / 16), dim3(256), 0, s, (const T*)x, ldx, m, k, codes, kpad, scale);
-  else hipLaunchKernelGGL((quantize_int8_kernel<T, V, 64>), dim3((m + 3) / 4), dim3(256), 0, s, (const T*)x, ldx, m, k, codes, kpad, scale);
+  auto launch = [&](auto kernel, int rows) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)m + rows - 1) / rows)), dim3(256), 0, s, (const T*)x, ldx, m, k,
+                       codes, kpad, scale);
+  };
+  if (vecs <= 32) launch(quantize_int8_kernel<T, V, 8>, 32);
+  else if (vecs <= 64) launch(quantize_int8_kernel<T, V, 16>, 16);
+  else launch(quantize_int8_kernel<T, V, 64>, 4);
 }
 
 template <typename T>
@@ -747,7 +761,7 @@ static int linear_run(Int8Args a, int8_t* codes, float* scale, hipStream_t s) {
   a.wide = a.act != LIC_ACT_GELU && p % 16 == 0 && a.ldy % E == 0 && (!a.r1 || a.ldr1 % E == 0);
   if (a.x) {
     const bool aligned = (uintptr_t)a.x % 16 == 0 && a.ldx % E == 0 && a.k % E == 0;
-    if (a.m <= ONE_TOKENS && a.kpad <= ONE_K) return aligned ? one_launch<T, 16 / sizeof(T)>(a, s) : one_launch<T, 1>(a, s);
+    if (a.m <= ONE_TOKENS && a.kpad <= ONE_K) return aligned ? one_launch<T, E>(a, s) : one_launch<T, 1>(a, s);
     // us, 192 -> 576 fp16 (quantised apart, tiles): 131072 tokens 54.4 (97), 16384: 16.0 (20.1), 8192: 13.4 (14.5), 4096: 12
     // (10); 384 -> 384: 79.5 (94); from kpad 448 on the operands spill; fp32, 192 -> 576: 32768 tokens 34 (45), 8192: 21 (17.5)
     if (aligned && a.m >= (sizeof(T) == 2 ? 8192 : 16384) && a.kpad <= 384 && a.wide && a.n % 32 == 0) return rows_run<T>(a, s);
@@ -755,8 +769,13 @@ static int linear_run(Int8Args a, int8_t* codes, float* scale, hipStream_t s) {
     a.xc = codes;
     a.xs = scale;
   }
+  // us, 4096 -> 4096 bf16, 16 / 64 tokens a workgroup / 64 x 64 tiles: 16 tokens 6.5 / 8.8 / -, 17: - / 8.9 / 12.9, 64: - /
+  // 12.5 / 12.9, 128: - / 21.2 / 13.2
   if (a.m <= 16) return few_launch<T, 1>(a, s);
   if (a.m <= 64) return few_launch<T, 4>(a, s);
+  // the largest tiles that give every compute unit one.  us, 256 x 256 / 128 x 128 / 64 x 64: 4096 x 2048 -> 4096 (256 of the
+  // largest) 44.7 / 51.9 / -, -> 2048 (128) 37.5 / 27.7 / -; 2048 x 2048 -> 2048 (256 of the middle) - / 16.5 / 20.3, -> 1024
+  // (128) - / 14.6 / 10.7
   const int64_t big = ((int64_t)a.m + 255) / 256 * ((a.n + 255) / 256);
   const int64_t mid = ((int64_t)a.m + 127) / 128 * ((a.n + 127) / 128);
   if (big >= 256) return tile_launch<T, 256, 256, 2, 4>(a, s);
@@ -796,7 +815,7 @@ extern "C" int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const 
                                void* y, int64_t ldy, void* ws, int64_t ws_bytes, lic_stream_t stream) {
   using namespace lic;
   if (check_sizes("linear_int8", dtype, m, k, kpad)) return 1;
-  if (n < 1) return fail("linear_int8: n out of range");
+  if (n < 1 || n > (1 << 30)) return fail("linear_int8: n out of range");
   if (act < LIC_ACT_NONE || act > LIC_ACT_GELU) return fail("linear_int8: act has to be none, relu, lrelu or gelu");
   if (m == 0) return 0;
   if (!w || !wscale || !y || ldy < n || (r1 && ldr1 < n)) return fail("linear_int8: null pointer or row stride below n");
@@ -806,7 +825,8 @@ extern "C" int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const 
   if (x) {
     if (ldx < k) return fail("linear_int8: row stride below k");
     const int64_t need = lic_linear_int8_workspace(m, kpad);
-    if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need)) return fail("linear_int8: workspace missing, misaligned or too small");
+    if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
+      return fail("linear_int8: workspace missing, misaligned or too small");
   }
   Int8Args a{xcodes, xscale, w, wscale, bias, r1, y, x, ldr1, ldy, ldx, m, n, k, kpad, act, slope, 0};
   int8_t* codes = (int8_t*)ws;

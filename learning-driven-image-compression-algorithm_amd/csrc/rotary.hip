@@ -64,7 +64,8 @@ enum RotaryForm { PARTNER, INSIDE, BOTH };
 
 // A block takes a few whole tokens: each angle's cos / sin once into LDS (all heads of the token share it), then the
 // tokens' vectors stream through, consecutive threads on consecutive vectors, ROTARY_UNROLL of them in flight a thread.
-// Bound by the bytes of x and y.
+// Bound by the bytes of x and y: 32 x 64 x 64 tokens of 384 fp16 channels 35 us (5.7 TB/s), 8 x 64 x 64 of 576 bf16 channels
+// with neighbouring pairs 13.9 us (5.4 TB/s); two tokens 2.8 us.
 template <typename T, int V, bool HALF, RotaryForm FORM>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float2 turn[];   // [tokens of the block][pairs]
