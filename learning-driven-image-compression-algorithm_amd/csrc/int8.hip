@@ -7,6 +7,9 @@
 namespace lic {
 
 template <typename T, int V> using QuantVec = T __attribute__((ext_vector_type(V)));
+// at any address: wide accesses need no alignment, those that cross a line cost two (4096 x 64 -> 4097 bf16, one element at a
+// time / 16 bytes: 61 / 46 us; -> 4098: 62 / 30)
+template <typename T, int V> using QuantLoose = T __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 
 // A row's codes: rint(127 x / top), half to even, exactly.  The fp32 product t = x * (127 / top) is within |t| 2^-22.4 of the
 // quotient.  16-bit x: a quotient that is no border k + 1/2 is at least |t| 2^-19 away from one (254 X - (2k + 1) T is a whole
@@ -107,29 +110,45 @@ template <> struct QuantMax<float> {
   static __device__ __forceinline__ float value(uint32_t b) { return b < 0x7f800000u ? __uint_as_float(b) : NAN; }
 };
 
+// Elements [j, j + V) of a row of k >= V, in reach of k: the vector that would pass the row's end is read where it ends, and its
+// codes are moved down by what it reads twice, which also leaves zeros behind k.
+template <typename T, int V>
+__device__ __forceinline__ QuantVec<T, V> quant_load(const T* x, int j, int k) {
+  if (j >= k) return QuantVec<T, V>{};
+  return *(const QuantLoose<T, V>*)(x + (j + V <= k ? j : k - V));
+}
+template <typename T, int V>
+__device__ __forceinline__ void quant_put(int8_t* to, const QuantVec<T, V>& u, int j, int k, const QuantRow& q) {
+  float f[V];
+  uint32_t w[(V + 3) / 4] = {};
+#pragma unroll
+  for (int e = 0; e < V; ++e) f[e] = to_f(u[e]);
+  if (q.inv != 0.f) quant_codes<T, V>(f, q, w);
+  const int twice = j < k && j + V > k ? 8 * (j + V - k) : 0;
+  if constexpr (V == 8) *(uint64_t*)(to + j) = (w[0] | (uint64_t)w[1] << 32) >> twice;
+  else if constexpr (V == 4) *(uint32_t*)(to + j) = w[0] >> twice;
+  else *(uint8_t*)(to + j) = (uint8_t)w[0];
+}
+
 // G lanes a row, V elements a load; a lane keeps its part of the row in registers (NV vectors of it; longer rows are read
-// a second time).  Bound by the bytes of x and codes: 8192 x 4096 bf16 21.5 us, 4.7 TB/s; 1037 x 333 fp32, whose
-// columns allow single elements only, 3.7 us.
+// a second time).  Bound by the bytes of x and codes: 8192 x 4096 bf16 21.5 us, 4.7 TB/s; 8192 x 4095
+// 22.6 (elements one by one: 49); 1037 x 333 fp32 2.9 us.
 template <typename T, int V, int G>
 __global__ __launch_bounds__(256) void quantize_int8_kernel(const T* __restrict__ x, int64_t ldx, int m, int k,
                                                             int8_t* __restrict__ codes, int kpad,
                                                             float* __restrict__ scale) {
-  constexpr int NV = V == 1 ? 8 : 4;
-  typedef QuantVec<T, V> Vec;
+  constexpr int NV = 4;
   const int lane = threadIdx.x & (G - 1);
   const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
   if (row >= m) return;
   const T* xr = x + row * ldx;
-  Vec v[NV];
+  QuantVec<T, V> v[NV];
   QuantMax<T> most;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    v[i] = Vec{};
-    if ((lane + i * G) * V < k) v[i] = *(const Vec*)(xr + (lane + i * G) * V);
-  }
+  for (int i = 0; i < NV; ++i) v[i] = quant_load<T, V>(xr, (lane + i * G) * V, k);
 #pragma unroll
   for (int i = 0; i < NV; ++i) most.add(v[i]);
-  for (int j = (lane + NV * G) * V; j < k; j += G * V) most.add(*(const Vec*)(xr + j));
+  for (int j = (lane + NV * G) * V; j < k; j += G * V) most.add(quant_load<T, V>(xr, j, k));
   uint32_t bits = most.bits();
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) {
@@ -139,30 +158,11 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(const T* __restrict_
   const float top = QuantMax<T>::value(bits);
   if (lane == 0) scale[row] = top / 127.f;
   const QuantRow q = quant_row(top);
-  typedef QuantVec<int8_t, V> Codes;
-  Codes* cr = (Codes*)(codes + row * kpad);
-  auto put = [&](const Vec& u, int j) {
-    float f[V];
-    uint32_t w[(V + 3) / 4];
-#pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = to_f(u[e]);
-    if (q.inv != 0.f) quant_codes<T, V>(f, q, w);
-    else
-#pragma unroll
-      for (int e = 0; e < (V + 3) / 4; ++e) w[e] = 0;
-    if constexpr (V == 8) *(uint2*)(cr + j / V) = make_uint2(w[0], w[1]);
-    else if constexpr (V == 4) *(uint32_t*)(cr + j / V) = w[0];
-    else if constexpr (V == 2) *(uint16_t*)(cr + j / V) = (uint16_t)w[0];
-    else *(uint8_t*)(cr + j / V) = (uint8_t)w[0];
-  };
+  int8_t* cr = codes + row * kpad;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if ((lane + i * G) * V < kpad) put(v[i], (lane + i * G) * V);   // columns behind k: zeros
-  for (int j = (lane + NV * G) * V; j < kpad; j += G * V) {
-    Vec u{};
-    if (j < k) u = *(const Vec*)(xr + j);
-    put(u, j);
-  }
+    if ((lane + i * G) * V < kpad) quant_put<T, V>(cr, v[i], (lane + i * G) * V, k, q);   // columns behind k: zeros
+  for (int j = (lane + NV * G) * V; j < kpad; j += G * V) quant_put<T, V>(cr, quant_load<T, V>(xr, j, k), j, k, q);
 }
 
 typedef int int32x4 __attribute__((ext_vector_type(4)));
@@ -181,7 +181,7 @@ struct Int8Args {
   int64_t ldr1, ldy, ldx;
   int32_t m, n, k, kpad, act;
   float slope;
-  int32_t wide;   // y, r1, ws and bias take 16-byte accesses at multiples of 16 columns; not GELU
+  int32_t wide;   // not GELU, whose many instructions would stand at every store
 };
 
 template <typename T>
@@ -193,11 +193,12 @@ __device__ __forceinline__ void int8_finish_one(const Int8Args& a, int64_t row, 
   ((T*)a.y)[row * a.ldy + col] = from_f<T>(u);
 }
 
-// N consecutive columns of one row, all inside y, aligned; not GELU.  ws, bias (or nullptr): those columns' own.
+// N consecutive columns of one row, all inside y (at any alignment); not GELU.  ws, bias (or nullptr): those columns' own.
 template <typename T, int N>
 struct Int8Out {
   static constexpr int E = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
   typedef QuantVec<T, E> Vec;
+  typedef QuantLoose<T, E> Loose;
   Vec o[N / E];
   __device__ __forceinline__ void compute(const Int8Args& a, int64_t row, int col, float xs, const int* acc,
                                           const float* ws, const float* bias) {
@@ -205,10 +206,10 @@ struct Int8Out {
     floatx4 b[N / 4] = {};
     if (bias)
 #pragma unroll
-      for (int e = 0; e < N / 4; ++e) b[e] = *(const floatx4*)(bias + 4 * e);
+      for (int e = 0; e < N / 4; ++e) b[e] = *(const QuantLoose<float, 4>*)(bias + 4 * e);
 #pragma unroll
     for (int e = 0; e < N / 4; ++e) {
-      const floatx4 w = *(const floatx4*)(ws + 4 * e);
+      const floatx4 w = *(const QuantLoose<float, 4>*)(ws + 4 * e);
 #pragma unroll
       for (int f = 0; f < 4; ++f) v[4 * e + f] = (float)acc[4 * e + f] * (xs * w[f]) + b[e][f];
     }
@@ -218,7 +219,7 @@ struct Int8Out {
       for (int e = 0; e < N; ++e) v[e] = v[e] > 0.f ? v[e] : (relu ? 0.f : v[e] * a.slope);
     }
     if (a.r1) {
-      const Vec* r = (const Vec*)((const T*)a.r1 + (row < a.m ? row : 0) * a.ldr1 + col);
+      const Loose* r = (const Loose*)((const T*)a.r1 + (row < a.m ? row : 0) * a.ldr1 + col);
 #pragma unroll
       for (int e = 0; e < N / E; ++e) {
         const Vec u = r[e];
@@ -233,7 +234,7 @@ struct Int8Out {
     if (row >= a.m) return;
     T* y = (T*)a.y + row * a.ldy + col;
 #pragma unroll
-    for (int e = 0; e < N / E; ++e) *(Vec*)(y + e * E) = o[e];
+    for (int e = 0; e < N / E; ++e) *(Loose*)(y + e * E) = o[e];
   }
 };
 
@@ -244,6 +245,7 @@ template <typename T>
 __device__ __forceinline__ void int8_tile_out(const Int8Args& a, int64_t m0, int n0, float xs, const int32x16& acc,
                                               int* stage, int lane) {
   const int row = lane & 31, half = lane >> 5;
+  if (m0 >= a.m || n0 >= a.n) return;
   if (a.wide && n0 + 32 <= a.n) {
     int v[16];
     const int col = n0 + 16 * half;
@@ -284,14 +286,17 @@ __device__ __forceinline__ int int8_channel(int r) {
 // in LDS, three of them in flight by LDS-DMA while one is multiplied (one barrier a step).  A row's four 16-byte chunks sit
 // at chunk ^ (row / 2) % 4: eight neighbouring lanes of a fragment read cover all 64 banks.  Bound by the matrix
 // instructions: 8192 x 4096 -> 8192 282 us, 1.95 POP/s (a large library product reaches 2.06); small ones by the latency of
-// their k steps: 128 x 4096 -> 4096 13.1 us, 1037 x 333 -> 517 fp32 8.9 us.
-template <typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int mt, int nt) {
+// their k steps, which KG groups of waves take a part of each and join in LDS: 128 x 4096 -> 4096 12.9 us with one, 9.9 with
+// two; 1037 x 333 -> 517 fp32 6.7 us.  More than four steps in flight gain nothing (128 x 4096 -> 4096 13.5 us with eight).
+template <typename T, int BM, int BN, int WM, int WN, int KG>
+__global__ __launch_bounds__(64 * WM * WN * KG) void int8_tile_kernel(Int8Args a, int mt, int nt) {
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, BK = 64, STAGES = 4;
+  static_assert(KG == 1 || TM * TN == 1, "groups join one tile a wave");
   constexpr int ROWS = BM + BN, LOADS = ROWS / 16 / NW;   // a wave's load: 16 rows of 64 bytes
   static_assert(ROWS % (16 * NW) == 0, "rows");
-  extern __shared__ __attribute__((aligned(1024))) int8_t smem[];   // [STAGES][BN weights, BM tokens][BK]
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  extern __shared__ __attribute__((aligned(1024))) int8_t lds[];   // [KG][STAGES][BN weights, BM tokens][BK]
+  const int lane = threadIdx.x & 63, id8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = id8 % NW, kg = id8 / NW;
+  int8_t* smem = lds + kg * STAGES * ROWS * BK;
   // workgroups go round the 8 XCDs: each gets a run of tiles, in groups of 8 token tiles that share their weights
   const int total = mt * nt, xcd = blockIdx.x & 7, per = total / 8, more = total & 7;
   const int id = xcd * per + min(xcd, more) + (int)(blockIdx.x >> 3);
@@ -300,13 +305,15 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
   const int64_t m0 = (int64_t)tm * BM;
   const int n0 = tn * BN;
 
+  // a group's steps of k; all of them meet at `most` barriers
+  const int whole = a.kpad / BK, s0 = whole * kg / KG, steps = whole * (kg + 1) / KG - s0, most = (whole + KG - 1) / KG;
   const int8_t* src[LOADS];
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) {
     const int r = (wave * LOADS + j) * 16 + (lane >> 2);
     const int chunk = (lane & 3) ^ ((r >> 1) & 3);
-    if (r < BN) src[j] = a.w + (int64_t)min(n0 + int8_channel(r), a.n - 1) * a.kpad + 16 * chunk;
-    else src[j] = a.xc + min(m0 + r - BN, (int64_t)a.m - 1) * a.kpad + 16 * chunk;
+    if (r < BN) src[j] = a.w + (int64_t)min(n0 + int8_channel(r), a.n - 1) * a.kpad + 16 * chunk + s0 * BK;
+    else src[j] = a.xc + min(m0 + r - BN, (int64_t)a.m - 1) * a.kpad + 16 * chunk + s0 * BK;
   }
   auto load = [&](int s) {
     int8_t* dst = smem + (s % STAGES) * ROWS * BK + wave * LOADS * 1024;
@@ -316,7 +323,6 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
                                        (int8_lds_void*)(dst + j * 1024), 16, 0, 0);
   };
   const int wm = wave % WM, wn = wave / WM;
-  const int steps = a.kpad / BK;
   int32x16 acc[TN][TM] = {};
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s)
@@ -360,17 +366,30 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, int
     __builtin_amdgcn_sched_barrier(0);
     multiply(0, 1, TM);
     __builtin_amdgcn_sched_barrier(0);
-    if (s + 1 < steps) {
+    if (s + 1 < most) {
       landed(s + 1);
       if (s + STAGES < steps) load(s + STAGES);
-      read(s + 1, 0);
+      if (KG == 1 || s + 1 < steps) read(s + 1, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
     multiply(1, 0, TM);
     __builtin_amdgcn_sched_barrier(0);
   }
   __syncthreads();   // the steps' buffers become the waves' staging
-  int* stage = (int*)smem + wave * INT8_STAGE;
+  int* stage = (int*)lds + wave * INT8_STAGE;
+  if constexpr (KG > 1) {
+    int* join = (int*)lds + NW * INT8_STAGE + wave * 1024 + lane;   // [KG - 1][NW][16][64]
+    if (kg) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) join[(kg - 1) * NW * 1024 + e * 64] = acc[0][0][e];
+    }
+    __syncthreads();
+    if (kg) return;
+#pragma unroll
+    for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[0][0][e] += join[g * NW * 1024 + e * 64];
+  }
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
     const int64_t token = m0 + (wm * TM + j) * 32 + row;
@@ -457,7 +476,6 @@ constexpr int ONE_TOKENS = 4, ONE_K = 4096;
 template <typename T, int V>
 __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
   constexpr int VECS = ONE_K / 512 / V;   // a thread's part of a row
-  typedef QuantVec<T, V> Vec;
   __shared__ int part[8][1][256];
   __shared__ uint32_t most[ONE_TOKENS][8];
   __shared__ float scale[ONE_TOKENS];
@@ -471,16 +489,14 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
 #pragma unroll
   for (int u = 0; u < 8; ++u)
     if (s0 + u < s1) fw[u] = *(const int32x4*)(w + 64 * (s0 + u));
-  Vec v[ONE_TOKENS][VECS];
+  QuantVec<T, V> v[ONE_TOKENS][VECS];
 #pragma unroll
   for (int r = 0; r < ONE_TOKENS; ++r) {
     if (r >= a.m) break;
     QuantMax<T> top;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      const int j = (threadIdx.x + 512 * i) * V;
-      v[r][i] = Vec{};
-      if (j < a.k) v[r][i] = *(const Vec*)((const T*)a.x + r * a.ldx + j);
+      v[r][i] = quant_load<T, V>((const T*)a.x + r * a.ldx, (threadIdx.x + 512 * i) * V, a.k);
       top.add(v[r][i]);
     }
     uint32_t bits = top.bits();
@@ -504,19 +520,7 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int j = (threadIdx.x + 512 * i) * V;
-      if (j < a.kpad) {
-        float f[V];
-        uint32_t c[(V + 3) / 4] = {};
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = to_f(v[r][i][e]);
-        if (qr.inv != 0.f) quant_codes<T, V>(f, qr, c);
-        if constexpr (V == 1) {
-          codes[r * a.kpad + j] = (int8_t)c[0];
-        } else {
-#pragma unroll
-          for (int e = 0; e < V / 4; ++e) ((uint32_t*)(codes + r * a.kpad + j))[e] = c[e];
-        }
-      }
+      if (j < a.kpad) quant_put<T, V>(codes + r * a.kpad, v[r][i], j, a.k, qr);
     }
   }
   __syncthreads();
@@ -532,7 +536,7 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
   int8_join<T, 1>(a, part, acc, n0, 0, scale);
 }
 
-// Many tokens of few channels (kpad = 64 KS; whole tiles of y only: n a multiple of 32, a.wide): 32 tokens a wave, quantised
+// Many tokens of few channels (kpad = 64 KS; whole tiles of y only: n a multiple of 32, aligned): 32 tokens a wave, quantised
 // straight into matrix operands that stay in registers; the weights pass through LDS, 64 channels at a time, the next under
 // way.  x is read once and y written once, the codes never reach memory.  Bound by the bytes of y: 131072 x 192 -> 576 fp16
 // 44 us alone, 53 with the call (201 MB; 35 without its stores).  A weight row's 16-byte chunks are placed so that a fragment
@@ -693,17 +697,19 @@ static int rows_run(const Int8Args& a, hipStream_t s) {
   }
 }
 
+// Rows of few vectors share a wave only where there are many: 1000 x 500 bf16 2.7 us with a wave a row, 3.5 with four rows a
+// wave; 131072 x 192 14.7 us with eight.
+constexpr int QUANT_FEW = 2048;
 template <typename T, int V>
 static void quantize_launch(const void* x, int64_t ldx, int m, int k, int8_t* codes, int kpad, float* scale,
                             hipStream_t s) {
   const int vecs = kpad / V;
-  // lanes of a row: up to four vectors each, a whole wave from there on
   auto launch = [&](auto kernel, int rows) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)m + rows - 1) / rows)), dim3(256), 0, s, (const T*)x, ldx, m, k,
                        codes, kpad, scale);
   };
-  if (vecs <= 32) launch(quantize_int8_kernel<T, V, 8>, 32);
-  else if (vecs <= 64) launch(quantize_int8_kernel<T, V, 16>, 16);
+  if (vecs <= 32 && m > QUANT_FEW) launch(quantize_int8_kernel<T, V, 8>, 32);
+  else if (vecs <= 64 && m > QUANT_FEW) launch(quantize_int8_kernel<T, V, 16>, 16);
   else launch(quantize_int8_kernel<T, V, 64>, 4);
 }
 
@@ -711,9 +717,7 @@ template <typename T>
 static int quantize_run(const void* x, int64_t ldx, int m, int k, int8_t* codes, int kpad, float* scale,
                         hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  auto fits = [&](int v) { return (uintptr_t)x % (v * sizeof(T)) == 0 && ldx % v == 0 && k % v == 0; };
-  if (fits(V)) quantize_launch<T, V>(x, ldx, m, k, codes, kpad, scale, s);
-  else if (fits(2)) quantize_launch<T, 2>(x, ldx, m, k, codes, kpad, scale, s);
+  if (k >= V) quantize_launch<T, V>(x, ldx, m, k, codes, kpad, scale, s);
   else quantize_launch<T, 1>(x, ldx, m, k, codes, kpad, scale, s);
   LIC_CHECK_LAUNCH();
   return 0;
@@ -726,14 +730,14 @@ static int quantize_any(int32_t dtype, const void* x, int64_t ldx, int m, int k,
   return quantize_run<bf16_t>(x, ldx, m, k, codes, kpad, scale, s);
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
+template <typename T, int BM, int BN, int WM, int WN, int KG>
 static int tile_launch(const Int8Args& a, hipStream_t s) {
   const int mt = (int)(((int64_t)a.m + BM - 1) / BM), nt = (a.n + BN - 1) / BN;
   if ((int64_t)mt * nt > INT32_MAX / 8) return fail("linear_int8: m x n out of range");
-  constexpr int LDS = 4 * (BM + BN) * 64;
-  const void* k = (const void*)int8_tile_kernel<T, BM, BN, WM, WN>;
+  constexpr int LDS = KG * 4 * (BM + BN) * 64;
+  const void* k = (const void*)int8_tile_kernel<T, BM, BN, WM, WN, KG>;
   if (ensure_dyn_lds(k, LDS) != hipSuccess) return fail("linear_int8: LDS limit");
-  hipLaunchKernelGGL((int8_tile_kernel<T, BM, BN, WM, WN>), dim3((unsigned)mt * nt), dim3(64 * WM * WN), LDS, s, a, mt,
+  hipLaunchKernelGGL((int8_tile_kernel<T, BM, BN, WM, WN, KG>), dim3((unsigned)mt * nt), dim3(64 * WM * WN * KG), LDS, s, a, mt,
                      nt);
   LIC_CHECK_LAUNCH();
   return 0;
@@ -758,29 +762,34 @@ template <typename T>
 static int linear_run(Int8Args a, int8_t* codes, float* scale, hipStream_t s) {
   const uintptr_t p = (uintptr_t)a.y | (uintptr_t)a.r1 | (uintptr_t)a.ws | (uintptr_t)a.bias;
   constexpr int E = 16 / sizeof(T);
-  a.wide = a.act != LIC_ACT_GELU && p % 16 == 0 && a.ldy % E == 0 && (!a.r1 || a.ldr1 % E == 0);
+  a.wide = a.act != LIC_ACT_GELU;
+  const bool lines = a.wide && p % 16 == 0 && a.ldy % E == 0 && (!a.r1 || a.ldr1 % E == 0);
   if (a.x) {
     const bool aligned = (uintptr_t)a.x % 16 == 0 && a.ldx % E == 0 && a.k % E == 0;
-    if (a.m <= ONE_TOKENS && a.kpad <= ONE_K) return aligned ? one_launch<T, E>(a, s) : one_launch<T, 1>(a, s);
+    if (a.m <= ONE_TOKENS && a.kpad <= ONE_K) return a.k >= E ? one_launch<T, E>(a, s) : one_launch<T, 1>(a, s);
     // us, 192 -> 576 fp16 (quantised apart, tiles): 131072 tokens 54.4 (97), 16384: 16.0 (20.1), 8192: 13.4 (14.5), 4096: 12
     // (10); 384 -> 384: 79.5 (94); from kpad 448 on the operands spill; fp32, 192 -> 576: 32768 tokens 34 (45), 8192: 21 (17.5)
-    if (aligned && a.m >= (sizeof(T) == 2 ? 8192 : 16384) && a.kpad <= 384 && a.wide && a.n % 32 == 0) return rows_run<T>(a, s);
+    if (aligned && a.m >= (sizeof(T) == 2 ? 8192 : 16384) && a.kpad <= 384 && lines && a.n % 32 == 0) return rows_run<T>(a, s);
     if (quantize_run<T>(a.x, a.ldx, a.m, a.k, codes, a.kpad, scale, s)) return 1;
     a.xc = codes;
     a.xs = scale;
   }
-  // us, 4096 -> 4096 bf16, 16 / 64 tokens a workgroup / 64 x 64 tiles: 16 tokens 6.5 / 8.8 / -, 17: - / 8.9 / 12.9, 64: - /
-  // 12.5 / 12.9, 128: - / 21.2 / 13.2
+  // us, 4096 -> 4096 bf16, 16 / 64 tokens a workgroup / 64 x 64 tiles: 16 tokens 6.5 / 8.8 / -, 17: - / 8.5 / 9.5, 32: - / 9.6 /
+  // 9.6, 64: - / 12.2 / 9.8; 64 x 1024 -> 1024: - / 4.6 / 4.8
   if (a.m <= 16) return few_launch<T, 1>(a, s);
-  if (a.m <= 64) return few_launch<T, 4>(a, s);
-  // the largest tiles that give every compute unit one.  us, 256 x 256 / 128 x 128 / 64 x 64: 4096 x 2048 -> 4096 (256 of the
-  // largest) 44.7 / 51.9 / -, -> 2048 (128) 37.5 / 27.7 / -; 2048 x 2048 -> 2048 (256 of the middle) - / 16.5 / 20.3, -> 1024
-  // (128) - / 14.6 / 10.7
-  const int64_t big = ((int64_t)a.m + 255) / 256 * ((a.n + 255) / 256);
-  const int64_t mid = ((int64_t)a.m + 127) / 128 * ((a.n + 127) / 128);
-  if (big >= 256) return tile_launch<T, 256, 256, 2, 4>(a, s);
-  if (mid >= 256) return tile_launch<T, 128, 128, 2, 2>(a, s);
-  return tile_launch<T, 64, 64, 2, 2>(a, s);
+  if (a.m <= 32 || (a.m <= 64 && a.kpad <= 1024)) return few_launch<T, 4>(a, s);
+  // Rounds of workgroups over 256 compute units: one with 256 x 256 tiles takes as long as 1 / 0.28 with 128 x 128 ones (two
+  // of which share a unit).  us, 256 x 256 / 128 x 128 / 64 x 64: 4096 x 2048 -> 4096 (256 of the largest) 44.7 / 51.9 / -,
+  // -> 4097 (272) 94.2 / 69.8 / -, -> 2048 (128) 37.5 / 27.7 / -; 2048 x 2048 -> 2048 (256 of the middle) - / 16.5 / 20.3,
+  // -> 1024 (128) - / 14.6 / 10.7
+  const int64_t big = ((int64_t)a.m + 255) / 256 * (((int64_t)a.n + 255) / 256);
+  const int64_t mid = ((int64_t)a.m + 127) / 128 * (((int64_t)a.n + 127) / 128);
+  if (big >= 256 && 100 * ((big + 255) / 256) <= 28 * ((mid + 255) / 256)) return tile_launch<T, 256, 256, 2, 4, 1>(a, s);
+  if (mid >= 256) return tile_launch<T, 128, 128, 2, 2, 1>(a, s);
+  // few tiles of a long k, 1 / 2 groups of waves: 128 x 4096 -> 4096 12.9 / 9.9 us, 1024 x 1024 -> 1024 5.8 / 5.3, 200 x 500 ->
+  // 1000 6.8 / 6.7; 2048 x 2048 -> 1024, of 512 tiles: 10.1 / 11.3
+  const int64_t small = ((int64_t)a.m + 63) / 64 * (((int64_t)a.n + 63) / 64);
+  return small <= 256 && a.kpad >= 1024 ? tile_launch<T, 64, 64, 2, 2, 2>(a, s) : tile_launch<T, 64, 64, 2, 2, 1>(a, s);
 }
 
 static int check_sizes(const char* who, int32_t dtype, int32_t m, int32_t k, int32_t kpad) {
