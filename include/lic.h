@@ -617,11 +617,12 @@ int lic_rotary(int32_t dtype, const void* x, int32_t ldx, int32_t n, int32_t h, 
  * the sum in 32-bit integers (k <= 131072 cannot overflow), the rest in fp32, rounded once to `dtype`.
  * Either xcodes / xscale ([m][kpad], fp32 [m]) or x (m rows of k, stride ldx, quantised by the call) is given.
  * act: LIC_ACT_NONE / RELU / LRELU / GELU; bias and r1 may be NULL; y must not overlap x, xcodes or w (r1 may
- * be y).  ws: with x, lic_linear_int8_workspace bytes, 16-byte aligned (0: up to 4 tokens of kpad <= 4096). */
+ * be y).  ws: with x, lic_linear_int8_workspace bytes, 16-byte aligned (0: small calls need none).  x, y, r1, wscale and
+ * bias may lie at any multiple of their elements' size. */
 #define LIC_INT8_MAX_K 131072
 int lic_quantize_int8(int32_t dtype, const void* x, int64_t ldx, int32_t m, int32_t k, int8_t* codes, int32_t kpad,
                       float* scale, lic_stream_t stream);
-int64_t lic_linear_int8_workspace(int32_t m, int32_t kpad);
+int64_t lic_linear_int8_workspace(int32_t m, int32_t kpad, int32_t n);
 int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const int8_t* xcodes, const float* xscale, int32_t m,
                     int32_t k, const int8_t* w, int32_t kpad, const float* wscale, const float* bias, int32_t n,
                     int32_t act, float slope, const void* r1, int64_t ldr1, void* y, int64_t ldy, void* ws,

@@ -305,7 +305,7 @@ def load():
                        ("lic_wgrad_reduce_blocks", [V])):
         getattr(lib, name).argtypes = argt
         getattr(lib, name).restype = ctypes.c_int32
-    for name, argt in (("lic_linear_int8_workspace", [I, I]), ("lic_orthogonalize_workspace", [I, I, V])):
+    for name, argt in (("lic_linear_int8_workspace", [I, I, I]), ("lic_orthogonalize_workspace", [I, I, V])):
         getattr(lib, name).argtypes = argt
         getattr(lib, name).restype = ctypes.c_int64
     lib.lic_last_error.restype = ctypes.c_char_p

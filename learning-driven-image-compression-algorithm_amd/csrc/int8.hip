@@ -3,6 +3,8 @@
 // The sum is an integer of 32 bits (exact, so no form or order of it shows in a result), the rest is fp32 and is rounded
 // once, to y's type.  The codes' 8 bits are the operator's definition.
 #include "lic_common.h"
+#include <algorithm>
+#include <type_traits>
 
 namespace lic {
 
@@ -110,33 +112,42 @@ template <> struct QuantMax<float> {
   static __device__ __forceinline__ float value(uint32_t b) { return b < 0x7f800000u ? __uint_as_float(b) : NAN; }
 };
 
-// Elements [j, j + V) of a row of k >= V, in reach of k: the vector that would pass the row's end is read where it ends, and its
-// codes are moved down by what it reads twice, which also leaves zeros behind k.
-template <typename T, int V>
-__device__ __forceinline__ QuantVec<T, V> quant_load(const T* x, int j, int k) {
-  if (j >= k) return QuantVec<T, V>{};
-  return *(const QuantLoose<T, V>*)(x + (j + V <= k ? j : k - V));
+// Elements [j, j + V) of a row, V those of 16 bytes: the vector that would pass the row's end is read where it ends, and its
+// codes are moved down by what it reads twice, which also leaves zeros behind k.  A row of less than one vector is gathered.
+template <typename T> constexpr int QUANT_V = 16 / sizeof(T);
+template <typename T>
+__device__ __forceinline__ QuantVec<T, QUANT_V<T>> quant_load(const T* x, int j, int k) {
+  constexpr int V = QUANT_V<T>;
+  typedef QuantVec<T, V> Vec;
+  if (j >= k) return Vec{};
+  if (k >= V) return *(const QuantLoose<T, V>*)(x + (j + V <= k ? j : k - V));
+  typedef std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t> Bits;
+  unsigned __int128 w = 0;
+#pragma nounroll
+  for (int e = k - 1; e >= 0; --e) w = w << 8 * sizeof(T) | __builtin_bit_cast(Bits, x[e]);
+  return __builtin_bit_cast(Vec, w);
 }
-template <typename T, int V>
-__device__ __forceinline__ void quant_put(int8_t* to, const QuantVec<T, V>& u, int j, int k, const QuantRow& q) {
+template <typename T>
+__device__ __forceinline__ void quant_put(int8_t* to, const QuantVec<T, QUANT_V<T>>& u, int j, int k, const QuantRow& q) {
+  constexpr int V = QUANT_V<T>;
   float f[V];
-  uint32_t w[(V + 3) / 4] = {};
+  uint32_t w[V / 4] = {};
 #pragma unroll
   for (int e = 0; e < V; ++e) f[e] = to_f(u[e]);
   if (q.inv != 0.f) quant_codes<T, V>(f, q, w);
-  const int twice = j < k && j + V > k ? 8 * (j + V - k) : 0;
-  if constexpr (V == 8) *(uint64_t*)(to + j) = (w[0] | (uint64_t)w[1] << 32) >> twice;
-  else if constexpr (V == 4) *(uint32_t*)(to + j) = w[0] >> twice;
-  else *(uint8_t*)(to + j) = (uint8_t)w[0];
+  const int twice = k >= V && j < k && j + V > k ? 8 * (j + V - k) : 0;
+  if constexpr (V == 8) *(uint64_t*)to = (w[0] | (uint64_t)w[1] << 32) >> twice;
+  else *(uint32_t*)to = w[0] >> twice;
 }
 
-// G lanes a row, V elements a load; a lane keeps its part of the row in registers (NV vectors of it; longer rows are read
+// G lanes a row; a lane keeps its part of the row in registers (NV vectors of it; longer rows are read
 // a second time).  Bound by the bytes of x and codes: 8192 x 4096 bf16 21.5 us, 4.7 TB/s; 8192 x 4095
 // 22.6 (elements one by one: 49); 1037 x 333 fp32 2.9 us.
-template <typename T, int V, int G>
+template <typename T, int G>
 __global__ __launch_bounds__(256) void quantize_int8_kernel(const T* __restrict__ x, int64_t ldx, int m, int k,
                                                             int8_t* __restrict__ codes, int kpad,
                                                             float* __restrict__ scale) {
+  constexpr int V = QUANT_V<T>;
   constexpr int NV = 4;
   const int lane = threadIdx.x & (G - 1);
   const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
@@ -145,10 +156,10 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(const T* __restrict_
   QuantVec<T, V> v[NV];
   QuantMax<T> most;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) v[i] = quant_load<T, V>(xr, (lane + i * G) * V, k);
+  for (int i = 0; i < NV; ++i) v[i] = quant_load<T>(xr, (lane + i * G) * V, k);
 #pragma unroll
   for (int i = 0; i < NV; ++i) most.add(v[i]);
-  for (int j = (lane + NV * G) * V; j < k; j += G * V) most.add(quant_load<T, V>(xr, j, k));
+  for (int j = (lane + NV * G) * V; j < k; j += G * V) most.add(quant_load<T>(xr, j, k));
   uint32_t bits = most.bits();
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) {
@@ -160,9 +171,11 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(const T* __restrict_
   const QuantRow q = quant_row(top);
   int8_t* cr = codes + row * kpad;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if ((lane + i * G) * V < kpad) quant_put<T, V>(cr, v[i], (lane + i * G) * V, k, q);   // columns behind k: zeros
-  for (int j = (lane + NV * G) * V; j < kpad; j += G * V) quant_put<T, V>(cr, quant_load<T, V>(xr, j, k), j, k, q);
+  for (int i = 0; i < NV; ++i) {
+    const int j = (lane + i * G) * V;
+    if (j < kpad) quant_put<T>(cr + j, v[i], j, k, q);   // columns behind k: zeros
+  }
+  for (int j = (lane + NV * G) * V; j < kpad; j += G * V) quant_put<T>(cr + j, quant_load<T>(xr, j, k), j, k, q);
 }
 
 typedef int int32x4 __attribute__((ext_vector_type(4)));
@@ -238,22 +251,39 @@ struct Int8Out {
   }
 };
 
-// A wave's 32 x 32 tile (lane: token m0 + lane % 32 with scale xs, channels n0 + 16 (lane / 32) ..): wide stores where the
-// tile lies inside y, else turned in the wave's LDS (INT8_STAGE words) so that 32 lanes meet consecutive channels.
+// A wave's 32 x 32 tile (lane: token m0 + lane % 32 with scale xs, channels n0 + 16 (lane / 32) ..): wide stores, one by one
+// where y's columns end inside a lane's; GELU is turned in the wave's LDS (INT8_STAGE words), so that its code stands once and
+// 32 lanes meet consecutive channels (so turned, the last columns cost 1 to 2 us more: 64 x 256 -> 1000 7.2 us for 6.1).
 constexpr int INT8_STAGE = 32 * 33;
 template <typename T>
 __device__ __forceinline__ void int8_tile_out(const Int8Args& a, int64_t m0, int n0, float xs, const int32x16& acc,
                                               int* stage, int lane) {
   const int row = lane & 31, half = lane >> 5;
   if (m0 >= a.m || n0 >= a.n) return;
-  if (a.wide && n0 + 32 <= a.n) {
-    int v[16];
+  if (a.wide) {
     const int col = n0 + 16 * half;
+    const int64_t token = m0 + row;
+    if (col + 16 <= a.n) {
+      int v[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = acc[e];
-    Int8Out<T, 16> out;
-    out.compute(a, m0 + row, col, xs, v, a.ws + col, a.bias ? a.bias + col : nullptr);
-    out.store(a, m0 + row, col);
+      for (int e = 0; e < 16; ++e) v[e] = acc[e];
+      Int8Out<T, 16> out;
+      out.compute(a, token, col, xs, v, a.ws + col, a.bias ? a.bias + col : nullptr);
+      out.store(a, token, col);
+    } else {
+      const T* r1 = (const T*)a.r1 + (token < a.m ? token : 0) * a.ldr1;
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int at = min(col + e, a.n - 1);
+        v[e] = (float)acc[e] * (xs * a.ws[at]) + (a.bias ? a.bias[at] : 0.f);
+        if (a.act != LIC_ACT_NONE) v[e] = v[e] > 0.f ? v[e] : (a.act == LIC_ACT_RELU ? 0.f : v[e] * a.slope);
+        if (a.r1) v[e] += to_f(r1[at]);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (token < a.m && col + e < a.n) ((T*)a.y)[token * a.ldy + col + e] = from_f<T>(v[e]);
+    }
     return;
   }
 #pragma unroll
@@ -287,7 +317,7 @@ __device__ __forceinline__ int int8_channel(int r) {
 // at chunk ^ (row / 2) % 4: eight neighbouring lanes of a fragment read cover all 64 banks.  Bound by the matrix
 // instructions: 8192 x 4096 -> 8192 282 us, 1.95 POP/s (a large library product reaches 2.06); small ones by the latency of
 // their k steps, which KG groups of waves take a part of each and join in LDS: 128 x 4096 -> 4096 12.9 us with one, 9.9 with
-// two; 1037 x 333 -> 517 fp32 6.7 us.  More than four steps in flight gain nothing (128 x 4096 -> 4096 13.5 us with eight).
+// two; 1037 x 333 -> 517 fp32 5.3 us.  More than four steps in flight gain nothing (128 x 4096 -> 4096 13.5 us with eight).
 template <typename T, int BM, int BN, int WM, int WN, int KG>
 __global__ __launch_bounds__(64 * WM * WN * KG) void int8_tile_kernel(Int8Args a, int mt, int nt) {
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, BK = 64, STAGES = 4;
@@ -473,9 +503,9 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
 // One to ONE_TOKENS tokens of up to ONE_K channels in one launch: every workgroup quantises them into LDS, its first weights
 // already under way.  Bound by latency, then the weights' bytes: 1 x 4096 -> 4096 7.5 us (quantised apart: 5.6 + 5.4).
 constexpr int ONE_TOKENS = 4, ONE_K = 4096;
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
-  constexpr int VECS = ONE_K / 512 / V;   // a thread's part of a row
+  constexpr int V = QUANT_V<T>, VECS = ONE_K / 512 / V;   // a thread's part of a row
   __shared__ int part[8][1][256];
   __shared__ uint32_t most[ONE_TOKENS][8];
   __shared__ float scale[ONE_TOKENS];
@@ -496,7 +526,7 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
     QuantMax<T> top;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      v[r][i] = quant_load<T, V>((const T*)a.x + r * a.ldx, (threadIdx.x + 512 * i) * V, a.k);
+      v[r][i] = quant_load<T>((const T*)a.x + r * a.ldx, (threadIdx.x + 512 * i) * V, a.k);
       top.add(v[r][i]);
     }
     uint32_t bits = top.bits();
@@ -520,7 +550,7 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int j = (threadIdx.x + 512 * i) * V;
-      if (j < a.kpad) quant_put<T, V>(codes + r * a.kpad, v[r][i], j, a.k, qr);
+      if (j < a.kpad) quant_put<T>(codes + r * a.kpad + j, v[r][i], j, a.k, qr);
     }
   }
   __syncthreads();
@@ -534,6 +564,75 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
     acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const int32x4*)(w + 64 * s), *(const int32x4*)(x + 64 * s), acc[0],
                                                    0, 0, 0);
   int8_join<T, 1>(a, part, acc, n0, 0, scale);
+}
+
+// Few tiles of up to FUSED_K channels in one launch: 32 tokens x 128 channels a workgroup.  Its weights are all asked for at
+// once (LDS-DMA), and while they come its tokens are quantised into LDS, sixteen lanes a token; then its 8 waves multiply, four
+// tiles of 32 x 32 in two halves of k that are joined in LDS.  Each of a token's tiles quantises it again.  us (two launches):
+// 64 x 192 -> 576 fp16 4.6 (5.5), 1037 x 333 -> 517 fp32 8.1 (8.4), 2500 x 192 -> 576 (395 tiles) 6.3 (7.8), fp32 8.0 (9.3),
+// 2000 x 384 -> 1000 fp32 (504) 12.7 (11.8), 4096 x 192 -> 576 (640) 7.9 (8.4), fp32 10.5 (10.8); and a call, a workspace less.
+constexpr int FUSED_K = 384, FUSED_M = 32, FUSED_N = 128, FUSED_TILES = 512;
+constexpr int FUSED_SUMS = 4 * (4096 + 4 * INT8_STAGE);   // four tiles of sums, then four waves' staging
+template <typename T>
+__global__ __launch_bounds__(512) void int8_fused_kernel(Int8Args a) {
+  constexpr int V = QUANT_V<T>, VECS = FUSED_K / 16 / V;
+  __shared__ float scale[FUSED_M];
+  extern __shared__ __attribute__((aligned(1024))) int8_t smem[];   // [FUSED_N weights, FUSED_M tokens][kpad], then the sums
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t m0 = (int64_t)blockIdx.y * FUSED_M;
+  const int n0 = blockIdx.x * FUSED_N, chunks = a.kpad / 16, ks = a.kpad / 64;
+  // where a row's 16-byte chunks are placed: a fragment read meets every bank once (rows advance by 16 ks of the 64 words)
+  const int shift = ks % 4 == 0 ? 0 : ks % 2 == 0 ? 1 : 2, mask = ks % 4 == 0 ? 15 : ks % 2 == 0 ? 7 : 3;
+  auto place = [&](int r, int c) { return c ^ ((r >> shift) & mask); };
+  const uint32_t inv = (1u << 22) / chunks + 1;   // g / chunks = g inv >> 22 for g < 4096, chunks from 4 to 64
+  for (int i = wave; i < FUSED_N / 64 * chunks; i += 8) {
+    const int g = i * 64 + lane, r = (int)((uint32_t)g * inv >> 22), p = g - r * chunks;
+    const int64_t ch = min(n0 + int8_channel(r), a.n - 1);
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.w + ch * a.kpad + 16 * place(r, p)),
+                                     (int8_lds_void*)(smem + i * 1024), 16, 0, 0);
+  }
+  const int r = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const T* x = (const T*)a.x + min(m0 + r, (int64_t)a.m - 1) * a.ldx;
+  QuantVec<T, V> v[VECS];
+  QuantMax<T> most;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) v[i] = quant_load<T>(x, (l + 16 * i) * V, a.k);
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) most.add(v[i]);
+  uint32_t bits = most.bits();
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    const uint32_t other = __shfl_xor(bits, o);
+    bits = other > bits ? other : bits;
+  }
+  const float top = QuantMax<T>::value(bits);
+  if (l == 0) scale[r] = top / 127.f;
+  const QuantRow q = quant_row(top);
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int j = (l + 16 * i) * V;
+    if (j < a.kpad) quant_put<T>(smem + (FUSED_N + r) * a.kpad + 16 * place(r, j / 16) + j % 16, v[i], j, a.k, q);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  const int row = lane & 31, half = lane >> 5, wn = wave & 3, part = wave >> 2;
+  const int8_t *wrow = smem + (wn * 32 + row) * a.kpad, *xrow = smem + (FUSED_N + row) * a.kpad;
+  int32x16 acc{};
+  for (int s = part; s < 2 * ks; s += 2) {
+    const int c = 16 * place(row, 2 * s + half);   // the same for rows 32 apart
+    acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const int32x4*)(wrow + c), *(const int32x4*)(xrow + c), acc, 0, 0, 0);
+  }
+  __syncthreads();   // the operands become sums and staging
+  int* join = (int*)smem + (wave & 3) * 1024 + lane;
+  if (part) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) join[e * 64] = acc[e];
+  }
+  __syncthreads();
+  if (part) return;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] += join[e * 64];
+  int8_tile_out<T>(a, m0, n0 + wn * 32, scale[row], acc, (int*)smem + 4096 + wave * INT8_STAGE, lane);
 }
 
 // Many tokens of few channels (kpad = 64 KS; whole tiles of y only: n a multiple of 32, aligned): 32 tokens a wave, quantised
@@ -700,25 +799,17 @@ static int rows_run(const Int8Args& a, hipStream_t s) {
 // Rows of few vectors share a wave only where there are many: 1000 x 500 bf16 2.7 us with a wave a row, 3.5 with four rows a
 // wave; 131072 x 192 14.7 us with eight.
 constexpr int QUANT_FEW = 2048;
-template <typename T, int V>
-static void quantize_launch(const void* x, int64_t ldx, int m, int k, int8_t* codes, int kpad, float* scale,
-                            hipStream_t s) {
-  const int vecs = kpad / V;
+template <typename T>
+static int quantize_run(const void* x, int64_t ldx, int m, int k, int8_t* codes, int kpad, float* scale,
+                        hipStream_t s) {
+  const int vecs = kpad / QUANT_V<T>;
   auto launch = [&](auto kernel, int rows) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)m + rows - 1) / rows)), dim3(256), 0, s, (const T*)x, ldx, m, k,
                        codes, kpad, scale);
   };
-  if (vecs <= 32 && m > QUANT_FEW) launch(quantize_int8_kernel<T, V, 8>, 32);
-  else if (vecs <= 64 && m > QUANT_FEW) launch(quantize_int8_kernel<T, V, 16>, 16);
-  else launch(quantize_int8_kernel<T, V, 64>, 4);
-}
-
-template <typename T>
-static int quantize_run(const void* x, int64_t ldx, int m, int k, int8_t* codes, int kpad, float* scale,
-                        hipStream_t s) {
-  constexpr int V = 16 / sizeof(T);
-  if (k >= V) quantize_launch<T, V>(x, ldx, m, k, codes, kpad, scale, s);
-  else quantize_launch<T, 1>(x, ldx, m, k, codes, kpad, scale, s);
+  if (vecs <= 32 && m > QUANT_FEW) launch(quantize_int8_kernel<T, 8>, 32);
+  else if (vecs <= 64 && m > QUANT_FEW) launch(quantize_int8_kernel<T, 16>, 16);
+  else launch(quantize_int8_kernel<T, 64>, 4);
   LIC_CHECK_LAUNCH();
   return 0;
 }
@@ -751,9 +842,21 @@ static int few_launch(const Int8Args& a, hipStream_t s) {
   return 0;
 }
 
-template <typename T, int V>
+static bool int8_fused(int64_t m, int32_t kpad, int64_t n) {
+  return kpad <= FUSED_K && (m + FUSED_M - 1) / FUSED_M * ((n + FUSED_N - 1) / FUSED_N) <= FUSED_TILES;
+}
+template <typename T>
+static int fused_launch(const Int8Args& a, hipStream_t s) {
+  const int lds = std::max((FUSED_M + FUSED_N) * a.kpad, FUSED_SUMS);   // below 64 KB
+  const dim3 tiles((a.n + FUSED_N - 1) / FUSED_N, (a.m + FUSED_M - 1) / FUSED_M);
+  hipLaunchKernelGGL(int8_fused_kernel<T>, tiles, dim3(512), lds, s, a);
+  LIC_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
 static int one_launch(const Int8Args& a, hipStream_t s) {
-  hipLaunchKernelGGL((int8_one_kernel<T, V>), dim3((a.n + 15) / 16), dim3(512), a.m * a.kpad, s, a);
+  hipLaunchKernelGGL(int8_one_kernel<T>, dim3((a.n + 15) / 16), dim3(512), a.m * a.kpad, s, a);
   LIC_CHECK_LAUNCH();
   return 0;
 }
@@ -766,16 +869,17 @@ static int linear_run(Int8Args a, int8_t* codes, float* scale, hipStream_t s) {
   const bool lines = a.wide && p % 16 == 0 && a.ldy % E == 0 && (!a.r1 || a.ldr1 % E == 0);
   if (a.x) {
     const bool aligned = (uintptr_t)a.x % 16 == 0 && a.ldx % E == 0 && a.k % E == 0;
-    if (a.m <= ONE_TOKENS && a.kpad <= ONE_K) return a.k >= E ? one_launch<T, E>(a, s) : one_launch<T, 1>(a, s);
+    if (a.m <= ONE_TOKENS && a.kpad <= ONE_K) return one_launch<T>(a, s);
     // us, 192 -> 576 fp16 (quantised apart, tiles): 131072 tokens 54.4 (97), 16384: 16.0 (20.1), 8192: 13.4 (14.5), 4096: 12
     // (10); 384 -> 384: 79.5 (94); from kpad 448 on the operands spill; fp32, 192 -> 576: 32768 tokens 34 (45), 8192: 21 (17.5)
     if (aligned && a.m >= (sizeof(T) == 2 ? 8192 : 16384) && a.kpad <= 384 && lines && a.n % 32 == 0) return rows_run<T>(a, s);
+    if (int8_fused(a.m, a.kpad, a.n)) return fused_launch<T>(a, s);
     if (quantize_run<T>(a.x, a.ldx, a.m, a.k, codes, a.kpad, scale, s)) return 1;
     a.xc = codes;
     a.xs = scale;
   }
-  // us, 4096 -> 4096 bf16, 16 / 64 tokens a workgroup / 64 x 64 tiles: 16 tokens 6.5 / 8.8 / -, 17: - / 8.5 / 9.5, 32: - / 9.6 /
-  // 9.6, 64: - / 12.2 / 9.8; 64 x 1024 -> 1024: - / 4.6 / 4.8
+  // us, 4096 -> 4096 bf16, 16 / 64 tokens a workgroup / 64 x 64 tiles: 16 tokens 6.5 / 8.8 / -, 17: - / 8.5 / 9.5, 32: - /
+  // 9.6 / 9.6, 64: - / 12.2 / 9.8; 64 x 1024 -> 1024: - / 4.6 / 4.8
   if (a.m <= 16) return few_launch<T, 1>(a, s);
   if (a.m <= 32 || (a.m <= 64 && a.kpad <= 1024)) return few_launch<T, 4>(a, s);
   // Rounds of workgroups over 256 compute units: one with 256 x 256 tiles takes as long as 1 / 0.28 with 128 x 128 ones (two
@@ -811,9 +915,9 @@ extern "C" int lic_quantize_int8(int32_t dtype, const void* x, int64_t ldx, int3
   return quantize_any(dtype, x, ldx, m, k, codes, kpad, scale, (hipStream_t)stream);
 }
 
-extern "C" int64_t lic_linear_int8_workspace(int32_t m, int32_t kpad) {
-  if (m < 0 || kpad < 1 || kpad > LIC_INT8_MAX_K) return -1;
-  if (m <= lic::ONE_TOKENS && kpad <= lic::ONE_K) return 0;   // quantised in LDS
+extern "C" int64_t lic_linear_int8_workspace(int32_t m, int32_t kpad, int32_t n) {
+  if (m < 0 || n < 1 || kpad < 1 || kpad > LIC_INT8_MAX_K) return -1;
+  if ((m <= lic::ONE_TOKENS && kpad <= lic::ONE_K) || lic::int8_fused(m, kpad, n)) return 0;   // quantised in LDS
   const int64_t codes = (int64_t)m * kpad;
   return (codes + 15) / 16 * 16 + 4 * (int64_t)m;
 }
@@ -833,7 +937,7 @@ extern "C" int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const 
   hipStream_t s = (hipStream_t)stream;
   if (x) {
     if (ldx < k) return fail("linear_int8: row stride below k");
-    const int64_t need = lic_linear_int8_workspace(m, kpad);
+    const int64_t need = lic_linear_int8_workspace(m, kpad, n);
     if (need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need))
       return fail("linear_int8: workspace missing, misaligned or too small");
   }

@@ -1241,6 +1241,13 @@ def pack_linear_int8(weight: torch.Tensor, bias: Optional[torch.Tensor] = None) 
     return Int8Pack(codes, scale, bias.detach().float().contiguous() if bias is not None else None, w.shape[1])
 
 
+def _int8_workspace(m: int, kpad: int, n: int) -> int:
+    """lic_linear_int8_workspace: nothing where a launch quantises in LDS."""
+    if (m <= 4 and kpad <= 4096) or (kpad <= 384 and -(-m // 32) * -(-n // 128) <= 512):
+        return 0
+    return -(-m * kpad // 16) * 16 + 4 * m
+
+
 def linear_int8(x, pk: Int8Pack, out: Optional[Act] = None, *, act: int = _ffi.ACT_NONE, slope: float = 0.01,
                 r1: Optional[Act] = None) -> Act:
     """act(x W^T + bias) + r1 per token of x (an Act, quantised by the call, or an Int8Act) in 8-bit products: integer
@@ -1269,8 +1276,7 @@ def linear_int8(x, pk: Int8Pack, out: Optional[Act] = None, *, act: int = _ffi.A
     m, kpad = B * H * W, pk.w.shape[1]
     if m == 0:
         return out
-    # lic_linear_int8_workspace
-    nbytes = 0 if q is not None or (m <= 4 and kpad <= 4096) else -(-m * kpad // 16) * 16 + 4 * m
+    nbytes = 0 if q is not None else _int8_workspace(m, kpad, co)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=src.device) if nbytes else None
     r1p, ldr1 = _ptr(r1)
     check(_lib().lic_linear_int8(dtype_id(dtype), None if q is not None else x.ptr, 0 if q is not None else x.ld,

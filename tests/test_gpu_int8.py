@@ -197,6 +197,31 @@ def test_linear_int8_few_tokens_any_alignment(dtype):
                 assert torch.equal(Fn.linear_int8(xa, pk).t, Fn.linear_int8(q, pk).t), (k, m, c0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_int8_one_launch(dtype):
+    """Few tiles of few channels, quantised inside the product: every row length around the vectors' and the steps', at odd
+    addresses, with a NaN row: the bits of the product of the codes made apart, which are exact."""
+    import lic_amd.functional as Fn
+    g = torch.Generator(device=DEV).manual_seed(6)
+    for k in (1, 2, 3, 4, 5, 7, 8, 9, 15, 63, 64, 65, 127, 190, 192, 250, 257, 320, 333, 383, 384, 385):
+        for m, n in ((5, 33), (64, 64), (70, 200), (333, 65)):
+            x = torch.randn(1, 1, m, k + 3, generator=g, device=DEV).to(dtype)
+            x[0, 0, 1, 1:] = 0
+            x[0, 0, 3, 1] = float("inf")
+            pk = Fn.pack_linear_int8(torch.randn(n, k, generator=g, device=DEV), torch.randn(n, generator=g, device=DEV))
+            r = Fn.Act(torch.randn(1, 1, m, n, generator=g, device=DEV).to(dtype))
+            xa = Fn.Act(x, 1, k)
+            q = Fn.quantize_tokens(xa)
+            ok = torch.ones(m, dtype=torch.bool, device=DEV)
+            ok[3] = False
+            codes, _ = _codes(x[0, 0, :, 1:1 + k][ok])
+            got = q.codes.view(m, -1)
+            assert torch.equal(got[ok][:, :k].double(), codes) and (got[:, k:] == 0).all() and (got[3] == 0).all()
+            y = Fn.linear_int8(xa, pk, act=2, r1=r).t
+            assert torch.isnan(y[0, 0, 3]).all() and torch.isfinite(y[0, 0, ok]).all()
+            assert torch.equal(y.nan_to_num(), Fn.linear_int8(q, pk, act=2, r1=r).t.nan_to_num()), (k, m, n)
+
+
 def test_linear_int8_rows_do_not_depend_on_the_batch():
     """Integer sums: a token's result is the same bits alone and in any batch, in every form the sizes select."""
     import lic_amd.functional as Fn

@@ -143,12 +143,17 @@ def test_c_entry_refusals():
     _refused(lin(x=None, xc=f), "x or xcodes")
     _refused(lin(w=f + 4), "aligned")
     _refused(lin(ldx=99), "stride below k")
-    _refused(lin(m=5, work=None), "workspace")
-    _refused(lin(m=5, work=f + 8), "workspace")
-    _refused(lin(m=5, nbytes=16), "workspace")
+    big = dict(m=5, k=400, ldx=400, kpad=448)
+    _refused(lin(work=None, **big), "workspace")
+    _refused(lin(work=f + 8, **big), "workspace")
+    _refused(lin(nbytes=16, **big), "workspace")
     assert lin(m=0) == 0
-    assert lib.lic_linear_int8_workspace(5, 128) >= 5 * 128 + 20 and lib.lic_linear_int8_workspace(-1, 128) == -1
-    assert lib.lic_linear_int8_workspace(4, 4096) == 0 and lib.lic_linear_int8_workspace(4, 4160) > 0
+    assert lib.lic_linear_int8_workspace(5, 448, 8) >= 5 * 448 + 20
+    assert lib.lic_linear_int8_workspace(-1, 128, 8) == -1 and lib.lic_linear_int8_workspace(1, 128, 0) == -1
+    for m in (1, 4, 5, 64, 65, 1037, 16384, 16385, 131072):
+        for kpad in (64, 384, 448, 4096, 4160):
+            for n in (1, 64, 65, 517, 16384):
+                assert lib.lic_linear_int8_workspace(m, kpad, n) == Fn._int8_workspace(m, kpad, n)
 
     def ortho(rows=8, cols=8, g=f, out=f, steps=5, eps=1e-7, dtype=0, count=1, ws=f, nbytes=1 << 30, coeffs=True):
         m = (_ffi.OrthoMat * 1)()
