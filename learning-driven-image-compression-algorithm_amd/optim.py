@@ -9,7 +9,7 @@ import torch.nn as nn
 
 from . import functional as Fn
 
-__all__ = ["Muon", "split_muon_params"]
+__all__ = ["Muon", "Together", "split_muon_params"]
 
 
 def split_muon_params(module: nn.Module, params: Iterable[torch.Tensor]) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:
@@ -43,12 +43,16 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("Muon: momentum in [0, 1), weight_decay >= 0")
         if adjust not in ("rms", "shape"):
             raise ValueError(f"Muon: adjust must be 'rms' or 'shape', got {adjust!r}")
+        if not 1 <= steps <= 64 or not eps >= 0:
+            raise ValueError("Muon: steps from 1 to 64, eps >= 0")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
                                       steps=steps, adjust=adjust, eps=eps))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2:
-                    raise ValueError("Muon: matrices and filters only (give vectors to another optimiser)")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        if any(p.dim() < 2 for p in self.param_groups[-1]["params"]):
+            del self.param_groups[-1]
+            raise ValueError("Muon: matrices and filters only (give vectors to another optimiser)")
 
     @staticmethod
     def _scale(adjust: str, rows: int, cols: int) -> float:
@@ -71,9 +75,10 @@ class Muon(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            params = [p for p in group["params"] if p.grad is not None]
+            params = [p for p in group["params"] if p.grad is not None and p.numel()]
             if not params:
                 continue
+            Fn._on_current_device("Muon", *params)
             lr, mu, wd = group["lr"], group["momentum"], group["weight_decay"]
             bufs = []
             for p in params:
@@ -87,7 +92,7 @@ class Muon(torch.optim.Optimizer):
             ups = torch._foreach_lerp(bufs, grads, 1.0 - mu) if group["nesterov"] else bufs
             mats = [u.reshape(u.shape[0], -1) for u in ups]
             orth = Fn.orthogonalize(mats, steps=group["steps"], eps=group["eps"])
-            orth = [o.view(p.shape).to(p.dtype) for o, p in zip(orth, params)]
+            orth = [o.view(p.shape) for o, p in zip(orth, params)]   # fp32: only the new weight is rounded to its type
             torch._foreach_mul_(orth, [self._scale(group["adjust"], *m.shape) for m in mats])
             if isinstance(lr, torch.Tensor):
                 torch._foreach_mul_(orth, lr)
@@ -99,3 +104,33 @@ class Muon(torch.optim.Optimizer):
                     torch._foreach_mul_(params, 1.0 - lr * wd)
                 torch._foreach_sub_(params, orth, alpha=lr)
         return loss
+
+
+class Together(torch.optim.Optimizer):
+    """Several optimisers as one: a GradScaler decides once whether the gradients are finite and all of them step or none,
+    and one scheduler sets every learning rate (the parameter groups are the optimisers' own)."""
+
+    def __init__(self, *optimizers: torch.optim.Optimizer):
+        if not optimizers:
+            raise ValueError("Together: at least one optimiser")
+        super().__init__([g for o in optimizers for g in o.param_groups], {})
+        self.optimizers = optimizers
+
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for o in self.optimizers:
+            o.step()
+        return loss
+
+    def state_dict(self):
+        return {"optimizers": [o.state_dict() for o in self.optimizers]}
+
+    def load_state_dict(self, state_dict):
+        if len(state_dict["optimizers"]) != len(self.optimizers):
+            raise ValueError("Together: a state of other optimisers")
+        for o, s in zip(self.optimizers, state_dict["optimizers"]):
+            o.load_state_dict(s)
+        self.param_groups = [g for o in self.optimizers for g in o.param_groups]

@@ -218,6 +218,20 @@ def test_muon_captured_step_matches_eager():
         assert all(torch.equal(p, q) for p, q in zip(eager, cap))
 
 
+def test_muon_16_bit_weights():
+    """bf16 weights move by the fp32 update and are rounded once; empty ones are left alone."""
+    from lic_amd.optim import Muon
+    g = torch.Generator().manual_seed(9)
+    w, grad = torch.randn(40, 64, generator=g).bfloat16(), torch.randn(40, 64, generator=g).bfloat16()
+    p, none = torch.nn.Parameter(w.to(DEV)), torch.nn.Parameter(torch.zeros(0, 8, device=DEV))
+    p.grad, none.grad = grad.to(DEV), torch.zeros(0, 8, device=DEV)
+    Muon([p, none], lr=0.1, momentum=0.0, adjust="shape").step()
+    want = w.double() - 0.1 * _newton_schulz(grad.double(), 5, C, 1e-7, torch.float64)
+    # the update's own error, 4 * 2.5e-6 of its norm, is below a value's rounding here
+    tol = torch.finfo(torch.bfloat16).eps / 2 * want.abs() + 0.1 * 1e-5 * math.sqrt(40)
+    assert ((p.detach().cpu().double() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("mode", ["--eager", "--graph"])
 def test_train_cli_with_muon(mode, monkeypatch, capsys):
     """train_net_unet.py --optimizer muon (at its 256 x 256 crops, which the net's windows need): eager and captured steps

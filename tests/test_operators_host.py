@@ -217,6 +217,41 @@ def test_muon_refusals_and_split():
         Muon(mats, lr=-1.0)
 
 
+def test_together_steps_all_or_none():
+    """One scheduler reaches every group, a state comes back whole, and a GradScaler that meets a NaN in one optimiser's
+    gradients leaves the other's weights alone too."""
+    from lic_amd.optim import Muon, Together
+    with pytest.raises(ValueError, match="at least one"):
+        Together()
+    p, q = (torch.nn.Parameter(torch.ones(3)) for _ in range(2))
+    opt = Together(torch.optim.Adam([p], lr=0.5), torch.optim.SGD([q], lr=0.25))
+    sch = torch.optim.lr_scheduler.MultiStepLR(opt, [1], 0.5)
+    p.grad, q.grad = torch.ones(3), torch.ones(3)
+    opt.step()
+    sch.step()
+    assert torch.allclose(p, torch.full((3,), 0.5)) and torch.equal(q, torch.full((3,), 0.75))
+    assert [o.param_groups[0]["lr"] for o in opt.optimizers] == [0.25, 0.125]
+    other = Together(torch.optim.Adam([p], lr=0.5), torch.optim.SGD([q], lr=0.25))
+    other.load_state_dict(opt.state_dict())
+    assert [g["lr"] for g in other.param_groups] == [0.25, 0.125] and other.optimizers[0].state[p]["step"] == 1
+    scaler = torch.amp.GradScaler("cpu", init_scale=4.0)
+    scaler.scale(torch.ones(()))
+    before = [p.detach().clone(), q.detach().clone()]
+    p.grad, q.grad = torch.tensor([1.0, float("nan"), 1.0]), torch.ones(3)
+    scaler.unscale_(opt)
+    scaler.step(opt)
+    scaler.update()
+    assert torch.equal(p, before[0]) and torch.equal(q, before[1])
+    opt.zero_grad(set_to_none=True)
+    assert p.grad is None and q.grad is None
+    m = Muon([torch.nn.Parameter(torch.zeros(4, 4))])
+    with pytest.raises(ValueError, match="matrices"):
+        m.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4))]})
+    assert len(m.param_groups) == 1
+    with pytest.raises(ValueError, match="steps"):
+        Muon([torch.nn.Parameter(torch.zeros(4, 4))], steps=0)
+
+
 def test_muon_state_keeps_fp32_momentum():
     from lic_amd.optim import Muon
     p = torch.nn.Parameter(torch.zeros(8, 8, dtype=torch.bfloat16))

@@ -146,13 +146,13 @@ def main():
 
     matrices, others = [], params
     if args.optimizer == "muon":
-        from lic_amd.optim import Muon, split_muon_params
+        from lic_amd.optim import Muon, Together, split_muon_params
         matrices, others = split_muon_params(net, params)
-    opts = [torch.optim.Adam(others, lr=learning_rate(), capturable=args.graph,
-                             fused=os.environ.get("LIC_FUSED_ADAM", "1") != "0")]
+    opt = torch.optim.Adam(others, lr=learning_rate(), capturable=args.graph,
+                           fused=os.environ.get("LIC_FUSED_ADAM", "1") != "0")
     if matrices:
-        opts.append(Muon(matrices, lr=learning_rate()))
-    schs = [torch.optim.lr_scheduler.MultiStepLR(o, [1500, 2500, 3500, 4000], 0.5) for o in opts]
+        opt = Together(opt, Muon(matrices, lr=learning_rate()))
+    sch = torch.optim.lr_scheduler.MultiStepLR(opt, [1500, 2500, 3500, 4000], 0.5)
     sync = D.GradAllReduce(params, world)
     # one GPU: the backward's split-K wgrad reduces as one launch after it (autograd.WgradDefer; at
     # world > 1 the eager GradAllReduce hooks read .grad during the backward).  LIC_WGRAD_DEFER=0: off
@@ -169,21 +169,13 @@ def main():
 
     grad_params = None
 
-    def zero_grad():
-        for o in opts:
-            o.zero_grad(set_to_none=True)
-
-    def opt_step():
-        for o in opts:
-            o.step()
-
     def step_body(x, seed_dev=None):
         bpp, mse = net(x, "train", seed_dev=seed_dev)
         loss = args.lmbda * 255 ** 2 * mse + bpp                       # :180
         backward(loss)
         sync.finish()                                                  # RCCL all-reduce, captured too
         torch.nn.utils.clip_grad_norm_(grad_params, 1.0)               # :198
-        opt_step()
+        opt.step()
         return loss.detach(), bpp.detach(), mse.detach()
 
     if args.graph:
@@ -198,17 +190,17 @@ def main():
         nwarm = max(2 if plan is not None else 1, args.warmup)
         with torch.cuda.stream(side):
             for k in range(nwarm):
-                zero_grad()
+                opt.zero_grad(set_to_none=True)
                 with plan.record() if (plan is not None and k == nwarm - 1) else contextlib.nullcontext():
                     bpp, mse = net(static_x, "train", seed_dev=seed_t)
                     backward(args.lmbda * 255 ** 2 * mse + bpp)
                 sync.finish()              # first collectives eagerly: communicator set up before capture
                 grad_params = [p for p in clip_params if p.grad is not None]
                 torch.nn.utils.clip_grad_norm_(grad_params, 1.0)
-                opt_step()
+                opt.step()
                 seed_t.add_(1)
         torch.cuda.current_stream().wait_stream(side)
-        zero_grad()
+        opt.zero_grad(set_to_none=True)
         if plan is not None:
             plan.finalize()
         torch.cuda.synchronize(dev)   # the warm-up's collectives complete before the capture starts
@@ -235,16 +227,14 @@ def main():
 
     def eager_step():
         x = batches()
-        zero_grad()
+        opt.zero_grad(set_to_none=True)
         bpp, mse = net(x, "train")
         loss = args.lmbda * 255 ** 2 * mse + bpp                       # :180
         backward(scaler.scale(loss))
         sync.finish()
-        for o in opts:
-            scaler.unscale_(o)
+        scaler.unscale_(opt)
         torch.nn.utils.clip_grad_norm_([p for p in clip_params if p.grad is not None], 1.0)   # :198
-        for o in opts:
-            scaler.step(o)
+        scaler.step(opt)
         scaler.update()
         return loss.detach(), bpp.detach(), mse.detach()
 
@@ -292,8 +282,7 @@ def main():
                     raise Exception("NaN in loss")                      # :189-190
                 sums = [s + v for s, v in zip(sums, vals)]
                 acc = None
-        for sch in schs:
-            sch.step()
+        sch.step()
         cnt = args.steps_per_epoch
         if rank == 0:
             msg = "[Epoch %04d TRAIN] Loss: %.4f bpp: %.4f mse: %.4f  " % (epoch, sums[0] / cnt, sums[1] / cnt,
