@@ -635,7 +635,8 @@ int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const int8_t* xco
  * 1e9.  Products of two fp16 parts each (22 bits), fp32 sums: the error of fp32 products.  A zero matrix
  * gives zeros, one with a NaN or an infinity nothing finite.  Deterministic (no atomics); a matrix's result
  * does not depend on its neighbours in the list.
- * ws: lic_orthogonalize_workspace bytes of device memory, 256-byte aligned, -1: sizes out of range. */
+ * ws: lic_orthogonalize_workspace bytes of device memory, 256-byte aligned, -1: sizes out of range (a shorter
+ * side above 65536, a longer one above 2^24, more than 2^30 tiles of 64 x 64 in all). */
 typedef struct lic_ortho_mat {
   const void* g; int64_t rs, cs;
   void* out;

@@ -491,9 +491,9 @@ static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 static bool ortho_plan(int count, const lic_ortho_mat* mats, OrthoPlan& p, OrthoDesc* d) {
   for (int i = 0; i < count; ++i) {
     const lic_ortho_mat& m = mats[i];
-    if (m.rows < 1 || m.cols < 1 || m.rows > 65536 || m.cols > (1 << 24)) return false;
     const bool flip = m.rows > m.cols;
     const int64_t r = flip ? m.cols : m.rows, c = flip ? m.rows : m.cols;
+    if (r < 1 || r > 65536 || c > (1 << 24)) return false;
     const int64_t nr = up(r, 64) / 64, nc = up(c, 64) / 64, x = nr * nc * 8192, a = nr * nr * 8192;   // halves, both parts
     if (nr * nc > (1 << 28)) return false;
     OrthoDesc o{m.g, m.out, flip ? m.cs : m.rs, flip ? m.rs : m.cs};

@@ -59,7 +59,7 @@ def test_orthogonalize_list(dtype):
         assert torch.equal(Fn.orthogonalize([a])[0], o)
 
 
-@pytest.mark.parametrize("m,n", [(700, 900), (1030, 520), (640, 640)])
+@pytest.mark.parametrize("m,n", [(700, 900), (1030, 520), (640, 640), (70000, 24), (24, 70000)])
 def test_orthogonalize_larger(m, n):
     import lic_amd.functional as Fn
     a = _gradient(m, n, torch.Generator().manual_seed(m), torch.float32).to(DEV)

@@ -161,7 +161,9 @@ def test_c_entry_refusals():
         co = (ctypes.c_float * 3)(*Fn.NEWTON_SCHULZ) if coeffs else None
         return lib.lic_orthogonalize(dtype, count, m, steps, co, eps, ws, nbytes, None)
     _refused(ortho(rows=0), "out of range")
-    _refused(ortho(rows=65537), "out of range")
+    _refused(ortho(rows=65537, cols=65537), "out of range")
+    _refused(ortho(rows=(1 << 24) + 1), "out of range")
+    _refused(ortho(cols=(1 << 24) + 1), "out of range")
     _refused(ortho(g=None), "null")
     _refused(ortho(out=None), "null")
     _refused(ortho(steps=0), "steps")
