@@ -59,12 +59,16 @@ struct OrthoBounds {
 
 __device__ __forceinline__ int ortho_tiles(int n) { return (n + 63) / 64; }
 
-__global__ __launch_bounds__(256) void ortho_setup_kernel(OrthoBatch b, int first, OrthoWork w) {
-  const OrthoDesc d = b.d[blockIdx.x];
-  const int mat = first + blockIdx.x, nr = ortho_tiles(d.r), nc = ortho_tiles(d.c), nu = (d.c + 255) / 256;
+// The tables' entries of one matrix, for the kernels that follow.
+__device__ __forceinline__ void ortho_setup(const OrthoDesc& d, int mat, const OrthoWork& w) {
+  const int nr = ortho_tiles(d.r), nc = ortho_tiles(d.c), nu = (d.c + 255) / 256;
   if (threadIdx.x == 0) w.desc[mat] = d;
   for (int i = threadIdx.x; i < nr * nc; i += 256) w.tiles[d.parts0 + i] = {mat, i};
-  for (int i = threadIdx.x; i < nr * nu; i += 256) w.upd[d.upd0 + i] = {mat, i};
+  // workgroups of one group of columns follow each other (in groups of 8 tiles of rows): they share X's fragments in the L2
+  for (int i = threadIdx.x; i < nr * nu; i += 256) {
+    const int group = i / (8 * nu), rest = i - group * 8 * nu, rows = min(8, nr - group * 8);
+    w.upd[d.upd0 + i] = {mat, (group * 8 + rest % rows) << 16 | rest / rows};
+  }
   for (int i = threadIdx.x; i < nr; i += 256)
     for (int j = 0; j <= i; ++j) {
       const int at = i * (i + 1) / 2 + j;
@@ -104,11 +108,18 @@ __device__ __forceinline__ void ortho_read(const OrthoDesc& d, int i0, int j0, F
 
 // Sums of squares in 64 bits: the squares of small gradients are below fp32's range.  A matrix without gaps is read as a
 // line, 4096 elements a workgroup.  Bound by G's bytes: 38 matrices of a codec's layers (42 MB) 12 us, 2048 x 2048 5.3 us.
+// The descriptors come in the launch's arguments, a batch of them at a time; a matrix's first workgroup also writes its
+// entries of the tables (128 x 576: 108.8 -> 107.6 us without a launch for them).
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoWork w) {
+__global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoBatch b, int count, int first, OrthoWork w) {
   __shared__ double red[4];
-  const OrthoTile t = w.tiles[blockIdx.x];
-  const OrthoDesc d = w.desc[t.mat];
+  const int id = b.d[0].parts0 + (int)blockIdx.x;
+  int m = 0;
+#pragma unroll
+  for (int i = 1; i < ORTHO_BATCH; ++i) m += i < count && b.d[i].parts0 <= id;
+  const OrthoDesc d = b.d[m];
+  const OrthoTile t{first + m, id - d.parts0};
+  if (t.at == 0) ortho_setup(d, t.mat, w);
   const int nc = ortho_tiles(d.c);
   double s = 0;
   if ((d.cs == 1 && d.rs == d.c) || (d.rs == 1 && d.cs == d.r)) {
@@ -135,7 +146,7 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoWork w) {
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) w.parts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+  if (threadIdx.x == 0) w.parts[id] = red[0] + red[1] + red[2] + red[3];
 }
 
 // value * 2^14 in two fp16 parts (|value| <= 1)
@@ -411,10 +422,8 @@ __global__ __launch_bounds__(256, 2) void ortho_update_kernel(OrthoWork w, int k
   const OrthoTile t = w.upd[ortho_id()];
   const OrthoDesc d = w.desc[t.mat];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nr = ortho_tiles(d.r), nc = ortho_tiles(d.c), nu = (d.c + 255) / 256;
-  // workgroups of one group of columns follow each other (in groups of 8 tiles of rows): they share X's fragments in the L2
-  const int group = t.at / (8 * nu), rest = t.at - group * 8 * nu, rows = min(8, nr - group * 8);
-  const int ti = group * 8 + rest % rows, tj = rest / rows * 4 + wave;
+  const int nr = ortho_tiles(d.r), nc = ortho_tiles(d.c);
+  const int ti = t.at >> 16, tj = (t.at & 0xffff) * 4 + wave;
   if (tj >= nc) return;
   const int64_t now = (k & 1) * d.step, next = d.step - now, tile = (int64_t)nr * 4 * 1024;
   floatx16 acc[2][2] = {};   // [tile of columns][tile of rows]
@@ -591,9 +600,8 @@ static int ortho_run(const OrthoPlan& p, int count, const lic_ortho_mat* mats, i
   for (int i = 0; i < count; i += ORTHO_BATCH) {   // offsets run on from batch to batch
     const int n = count - i < ORTHO_BATCH ? count - i : ORTHO_BATCH;
     if (!ortho_plan(n, mats + i, q, b.d)) return fail("orthogonalize: sizes out of range");
-    hipLaunchKernelGGL(ortho_setup_kernel, dim3(n), dim3(256), 0, s, b, i, w);
+    hipLaunchKernelGGL(ortho_norm_kernel<T>, dim3((unsigned)(q.parts - b.d[0].parts0)), dim3(256), 0, s, b, n, i, w);
   }
-  hipLaunchKernelGGL(ortho_norm_kernel<T>, dim3((unsigned)p.parts), dim3(256), 0, s, w);
   hipLaunchKernelGGL(ortho_scale_kernel<T>, dim3((unsigned)p.parts), dim3(256), 0, s, w, bounds, steps, eps);
   for (int k = 0; k < steps; ++k) {
     hipLaunchKernelGGL(ortho_gram_kernel<0>, dim3((unsigned)p.slices), dim3(256), 0, s, w, k, 0.f, 0.f, 0.f, 0);
