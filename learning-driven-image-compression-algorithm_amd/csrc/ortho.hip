@@ -33,6 +33,7 @@ struct OrthoDesc {
   int32_t slices;       // workgroups that share a tile of A = X X^T
   int32_t slice0, sum0; // first of them, and of the tiles that are summed up from more than one
   int32_t partial0;     // first of the slices' sums
+  int64_t rest;         // both copies' third parts of X^T (fine matrices only, else -1)
 };
 
 // The workgroups of a stage in matrix order.
@@ -107,7 +108,7 @@ __device__ __forceinline__ void ortho_read(const OrthoDesc& d, int i0, int j0, F
 }
 
 // Sums of squares in 64 bits: the squares of small gradients are below fp32's range.  A matrix without gaps is read as a
-// line, 4096 elements a workgroup.  Bound by G's bytes: 38 matrices of a codec's layers (42 MB) 12 us, 2048 x 2048 5.3 us.
+// line, 4096 elements a workgroup.  Bound by G's bytes: 42 matrices of a codec's layers (42 MB) 12 us, 2048 x 2048 5.3 us.
 // The descriptors come in the launch's arguments, a batch of them at a time; a matrix's first workgroup also writes its
 // entries of the tables (128 x 576: 108.8 -> 107.6 us without a launch for them).
 template <typename T>
@@ -150,11 +151,12 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoBatch b, int count
 }
 
 // value * 2^14 in two fp16 parts (|value| <= 1)
-struct OrthoParts { half8 hi, lo; };
+struct OrthoParts { half8 hi, lo, rest; };
 __device__ __forceinline__ void ortho_split(OrthoParts& p, int e, float scaled) {
   const half_t h = (half_t)scaled;
   p.hi[e] = h;
   p.lo[e] = (half_t)(scaled - (float)h);
+  p.rest[e] = (half_t)(scaled - (float)h - (float)p.lo[e]);   // fine matrices'
 }
 
 // The fragments of a 64 x 64 tile in LDS (t[row][col], `flip`: its transpose): thread (of 512) -> 8 values of k.
@@ -170,13 +172,16 @@ __device__ __forceinline__ OrthoParts ortho_gather(const float* t, int rowtile, 
 __device__ __forceinline__ half_t* ortho_fragment(half_t* m, int ksteps, int rowtile, int ks) {
   return m + ((int64_t)rowtile * ksteps + ks) * 1024;
 }
+__device__ __forceinline__ half_t* ortho_third(half_t* m, int ksteps, int rowtile, int ks, int lane) {
+  return m + ((int64_t)rowtile * ksteps + ks) * 512 + lane * 8;
+}
 __device__ __forceinline__ void ortho_put(half_t* frag, int lane, const OrthoParts& p) {
   *(half8*)(frag + lane * 8) = p.hi;
   *(half8*)(frag + 512 + lane * 8) = p.lo;
 }
 
 // X = G / (|G| + eps) in both orders; the exponents of all steps' scales.  Bound by the bytes of G and of both copies (12 a
-// fp32 element): 2048 x 2048 16.3 us (3.1 TB/s), the 38 matrices 28 us (4.4 TB/s).
+// fp32 element): 2048 x 2048 16.3 us (3.1 TB/s), the 42 matrices 28 us (4.4 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_scale_kernel(OrthoWork w, OrthoBounds b, int steps, float eps) {
   __shared__ double red[4];
@@ -214,7 +219,9 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(OrthoWork w, OrthoBoun
   for (int u = 0; u < 2; ++u) {
     const int f = wave * 2 + u, rt = f >> 2, ks = f & 3;
     ortho_put(ortho_fragment(x, nc * 4, i0 * 2 + rt, j0 * 4 + ks), lane, ortho_gather<false>(tile, rt, ks, lane, 1.f));
-    ortho_put(ortho_fragment(xt, nr * 4, j0 * 2 + rt, i0 * 4 + ks), lane, ortho_gather<true>(tile, rt, ks, lane, 1.f));
+    const OrthoParts pt = ortho_gather<true>(tile, rt, ks, lane, 1.f);
+    ortho_put(ortho_fragment(xt, nr * 4, j0 * 2 + rt, i0 * 4 + ks), lane, pt);
+    if (d.rest >= 0) *(half8*)ortho_third(w.ops + d.rest, nr * 4, j0 * 2 + rt, i0 * 4 + ks, lane) = pt.rest;
   }
 }
 
@@ -287,6 +294,35 @@ __device__ __forceinline__ void ortho_product(floatx16 (&sum)[2][2], const half_
     }
     ortho_sum(sum, acc);
   }
+}
+
+// What two parts leave out of Q X, for matrices whose short sums would show it: Q's low part with X's, Q's high part with X's
+// third, which is what fp32 holds of X beyond 22 bits.  The error against 64 bits is mostly that of X between the steps; 2-norm
+// against that of fp32 products: 16 x 144 1.20 -> 0.81 of it, 64 x 64 1.25 -> 1.02; 66 x 66, without, 1.24, 128 x 128 1.13,
+// 192 x 192 1.01, where the sums' own rounding is as large.  64 x 576 91.9 -> 103.3 us; up to 128 rows 128 x 576 would be 135.
+constexpr int ORTHO_FINE = 64;
+__device__ __forceinline__ void ortho_finer(floatx16 (&sum)[2][2], const half_t* x, const half_t* rest, const half_t* q,
+                                            int64_t tile) {
+  floatx16 acc[2][2] = {};
+#pragma unroll
+  for (int s = 0; s < ORTHO_FINE / 16; ++s) {   // all of the sum
+    half8 lo[2], third[2], qh[2], ql[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      lo[i] = *(const half8*)(x + i * tile + (int64_t)s * 1024 + 512);
+      third[i] = *(const half8*)(rest + i * tile / 2 + (int64_t)s * 512);
+      qh[i] = *(const half8*)(q + i * tile + (int64_t)s * 1024);
+      ql[i] = *(const half8*)(q + i * tile + (int64_t)s * 1024 + 512);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo[i], ql[j], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(third[i], qh[j], acc[i][j], 0, 0, 0);
+      }
+  }
+  ortho_sum(sum, acc);
 }
 
 // A 64 x 64 tile of the lower triangle of A = X X^T (STAGE 0) or Q = a I + b A + c A A (STAGE 1), and its mirror image, from
@@ -415,7 +451,7 @@ __device__ __forceinline__ void ortho_out(OrthoGlobal<T> out, int count, bool wi
 // X <- Q X: 64 rows x 64 columns a wave, 64 x 256 a workgroup (Q's fragments are shared through the L1).  The last step
 // writes the result instead.  Bound by the matrix instructions and the 8 bytes an element of both copies: 2048 x 2048 59 us,
 // 873 TFLOP/s of fp16 products (the library's large fp16 product: 1160; operands through LDS in 128 x 128 tiles: 68 us;
-// 128 x 256 a workgroup: 93); the 38 matrices, whose sums are 1 to 32 k steps long, 35 us for 123 MB.
+// 128 x 256 a workgroup: 93); the 42 matrices, whose sums are 1 to 32 k steps long, 35 us for 123 MB.
 template <typename T>
 __global__ __launch_bounds__(256, 2) void ortho_update_kernel(OrthoWork w, int k, int last, int qexp) {
   __shared__ float turn[4][32 * 33];
@@ -429,6 +465,10 @@ __global__ __launch_bounds__(256, 2) void ortho_update_kernel(OrthoWork w, int k
   floatx16 acc[2][2] = {};   // [tile of columns][tile of rows]
   ortho_product(acc, w.ops + d.xt + now + tj * 2 * tile + lane * 8, w.ops + d.q + ti * 2 * tile + lane * 8, tile, tile, 0,
                 nr * 4);
+  if (d.rest >= 0)
+    ortho_finer(acc, w.ops + d.xt + now + tj * 2 * tile + lane * 8,
+                ortho_third(w.ops + d.rest + (k & 1) * (int64_t)nr * nc * 4096, nr * 4, tj * 2, 0, lane),
+                w.ops + d.q + ti * 2 * tile + lane * 8, tile);
   const int32_t* ex = w.exps + t.mat * (ORTHO_MAX_STEPS + 1) + k;
   const int half = lane >> 5, place = ortho_place(lane & 31);
   // the sum carries 2^28, Q's and X's scales
@@ -478,6 +518,9 @@ __global__ __launch_bounds__(256, 2) void ortho_update_kernel(OrthoWork w, int k
           }
           ortho_put(fx, (lane & 31) + 32 * h, px);
           ortho_put(ft, (lane & 31) + 32 * h, pt);
+          if (d.rest >= 0)
+            *(half8*)ortho_third(w.ops + d.rest + (1 - (k & 1)) * (int64_t)nr * nc * 4096, nr * 4, tj * 2 + j,
+                                 ti * 4 + i * 2 + half, (lane & 31) + 32 * h) = pt.rest;
         }
       }
     }
@@ -515,6 +558,8 @@ static bool ortho_plan(int count, const lic_ortho_mat* mats, OrthoPlan& p, Ortho
     o.a = o.x + 4 * x;
     o.q = o.a + a;
     p.halves = o.q + a;
+    o.rest = r <= ORTHO_FINE ? p.halves : -1;
+    if (r <= ORTHO_FINE) p.halves += x;   // two copies of half as much as X's two parts
     o.parts0 = (int32_t)p.parts;
     o.gram0 = (int32_t)p.gram;
     o.upd0 = (int32_t)p.upd;
