@@ -108,7 +108,8 @@ __device__ __forceinline__ void ortho_read(const OrthoDesc& d, int i0, int j0, F
 }
 
 // Sums of squares in 64 bits: the squares of small gradients are below fp32's range.  A matrix without gaps is read as a
-// line, 4096 elements a workgroup.  Bound by G's bytes: 42 matrices of a codec's layers (42 MB) 12 us, 2048 x 2048 5.3 us.
+// line, 4096 elements a workgroup.  Bound by G's bytes: 42 matrices of a codec's layers (42 MB)
+// 19 us in two launches, tables included (12 without them), 2048 x 2048 7.8 us (5.3).
 // The descriptors come in the launch's arguments, a batch of them at a time; a matrix's first workgroup also writes its
 // entries of the tables (128 x 576: 108.8 -> 107.6 us without a launch for them).
 template <typename T>
