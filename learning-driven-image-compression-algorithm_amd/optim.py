@@ -108,13 +108,28 @@ class Muon(torch.optim.Optimizer):
 
 class Together(torch.optim.Optimizer):
     """Several optimisers as one: a GradScaler decides once whether the gradients are finite and all of them step or none,
-    and one scheduler sets every learning rate (the parameter groups are the optimisers' own)."""
+    and one scheduler sets every learning rate.  The parameter groups are the optimisers' own, those that one of them is
+    given later included."""
 
     def __init__(self, *optimizers: torch.optim.Optimizer):
         if not optimizers:
             raise ValueError("Together: at least one optimiser")
         super().__init__([g for o in optimizers for g in o.param_groups], {})
         self.optimizers = optimizers
+        del self._at_first
+
+    @property
+    def param_groups(self):
+        return [g for o in self.optimizers for g in o.param_groups] if "optimizers" in self.__dict__ else self._at_first
+
+    @param_groups.setter
+    def param_groups(self, groups):   # the base class' list while it checks the optimisers' groups against each other
+        self._at_first = groups
+
+    def add_param_group(self, param_group):
+        if "optimizers" in self.__dict__:
+            raise ValueError("Together: give the group to one of its optimisers (optimizers[i].add_param_group)")
+        super().add_param_group(param_group)
 
     def step(self, closure=None):
         loss = None
@@ -133,4 +148,3 @@ class Together(torch.optim.Optimizer):
             raise ValueError("Together: a state of other optimisers")
         for o, s in zip(self.optimizers, state_dict["optimizers"]):
             o.load_state_dict(s)
-        self.param_groups = [g for o in self.optimizers for g in o.param_groups]

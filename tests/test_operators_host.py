@@ -285,3 +285,29 @@ def test_rotary_block_refusal():
         WinBasedAttention(24, 8, 8, rotary=100.0)
     plain, turned = WinBasedAttention(32, 4, 8), WinBasedAttention(32, 4, 8, rotary=100.0)
     assert plain.state_dict().keys() == turned.state_dict().keys()
+
+
+def test_together_takes_no_groups_of_its_own():
+    """A group that no optimiser would step is refused; one given to an optimiser is stepped, and the whole's scheduler,
+    zero_grad and GradScaler see it."""
+    from lic_amd.optim import Together
+    p, q, r = (torch.nn.Parameter(torch.ones(3)) for _ in range(3))
+    opt = Together(torch.optim.Adam([p], lr=0.5), torch.optim.SGD([q], lr=0.25))
+    with pytest.raises(ValueError, match="one of its optimisers"):
+        opt.add_param_group({"params": [r]})
+    assert len(opt.param_groups) == 2
+    opt.optimizers[1].add_param_group({"params": [r], "lr": 0.5})
+    assert [g["lr"] for g in opt.param_groups] == [0.5, 0.25, 0.5] and opt.param_groups[2]["params"][0] is r
+    sch = torch.optim.lr_scheduler.MultiStepLR(opt, [1], 0.5)
+    r.grad = torch.ones(3)
+    opt.step()
+    sch.step()
+    assert torch.equal(r, torch.full((3,), 0.5)) and opt.optimizers[1].param_groups[1]["lr"] == 0.25
+    scaler = torch.amp.GradScaler("cpu", init_scale=4.0)
+    scaler.scale(torch.ones(()))
+    scaler.unscale_(opt)
+    assert torch.equal(r.grad, torch.full((3,), 0.25))
+    opt.zero_grad(set_to_none=True)
+    assert r.grad is None
+    with pytest.raises(ValueError, match="more than one"):
+        Together(torch.optim.SGD([p], lr=0.1), torch.optim.SGD([p], lr=0.1))
