@@ -126,6 +126,9 @@ class Together(torch.optim.Optimizer):
     def param_groups(self, groups):   # the base class' list while it checks the optimisers' groups against each other
         self._at_first = groups
 
+    def __getstate__(self):   # copies and pickles: the groups are in the optimisers
+        return {"defaults": self.defaults, "state": self.state, "optimizers": self.optimizers}
+
     def add_param_group(self, param_group):
         if "optimizers" in self.__dict__:
             raise ValueError("Together: give the group to one of its optimisers (optimizers[i].add_param_group)")

@@ -311,3 +311,29 @@ def test_together_takes_no_groups_of_its_own():
     assert r.grad is None
     with pytest.raises(ValueError, match="more than one"):
         Together(torch.optim.SGD([p], lr=0.1), torch.optim.SGD([p], lr=0.1))
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+def test_together_copies_whole(how):
+    """A copy steps its own parameters with its own optimisers, whose groups and state are the copy's."""
+    import copy
+    import pickle
+    from lic_amd.optim import Together
+    p, q = (torch.nn.Parameter(torch.ones(3)) for _ in range(2))
+    opt = Together(torch.optim.Adam([p], lr=0.5), torch.optim.SGD([q], lr=0.25, momentum=0.5))
+    p.grad, q.grad = torch.ones(3), torch.ones(3)
+    opt.step()
+    twin = copy.deepcopy(opt) if how == "deepcopy" else pickle.loads(pickle.dumps(opt))
+    assert [type(o) for o in twin.optimizers] == [torch.optim.Adam, torch.optim.SGD]
+    (p2,), (q2,) = (g["params"] for g in twin.param_groups)
+    assert p2 is not p and torch.equal(p2, p) and torch.equal(q2, q)
+    assert twin.optimizers[0].state[p2]["step"] == 1
+    p2.grad, q2.grad = torch.ones(3), torch.ones(3)
+    torch.optim.lr_scheduler.MultiStepLR(twin, [1], 0.5)
+    for g in twin.param_groups:
+        g["lr"] = 0.125
+    twin.step()
+    assert torch.equal(q2, torch.full((3,), 0.75 - 0.125 * 1.5)) and torch.equal(q, torch.full((3,), 0.75))
+    assert [g["lr"] for g in opt.param_groups] == [0.5, 0.25] and twin.optimizers[0].state[p2]["step"] == 2
+    twin.load_state_dict(opt.state_dict())
+    assert [g["lr"] for g in twin.param_groups] == [0.5, 0.25]
