@@ -87,12 +87,13 @@ class WinBasedAttention(nn.Module):
                                     qkv_bias=qkv_bias, qk_scale=qk_scale, attn_drop=attn_drop, proj_drop=drop)
 
     def rotary_plan(self, device) -> Fn.RotaryPlan:
-        """The q / k rotation's plan on a device (kept: it holds only constants)."""
+        """The q / k rotation's plan on a device (kept for what it is made of: it holds only constants)."""
         plans = self.__dict__.setdefault("_rotary_plans", {})
-        if device not in plans:
-            d = self.dim // self.num_heads
-            plans[device] = Fn.RotaryPlan(d, (d // 4, d // 2 - d // 4), base=self.rotary, device=device)
-        return plans[device]
+        d = self.dim // self.num_heads
+        key = device, self.rotary, d
+        if key not in plans:
+            plans[key] = Fn.RotaryPlan(d, (d // 4, d // 2 - d // 4), base=self.rotary, device=device)
+        return plans[key]
 
     def run(self, x: Act, out: Optional[Act] = None, **proj_kw) -> Act:
         """out = x + proj(attention(qkv(x))); extra epilogue kwargs go to the proj launch.  Under fp32x6

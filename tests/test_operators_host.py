@@ -337,3 +337,21 @@ def test_together_copies_whole(how):
     assert [g["lr"] for g in opt.param_groups] == [0.5, 0.25] and twin.optimizers[0].state[p2]["step"] == 2
     twin.load_state_dict(opt.state_dict())
     assert [g["lr"] for g in twin.param_groups] == [0.5, 0.25]
+
+
+def test_rotary_plan_follows_the_block():
+    """The plan is that of the block's present base and heads, also after a run with others; equal ones are kept."""
+    from lic_amd.layers import WinBasedAttention
+    blk = WinBasedAttention(32, 4, 8, rotary=100.0)
+    first = blk.rotary_plan("cpu")
+    assert blk.rotary_plan("cpu") is first
+    blk.rotary = 10000.0
+    fresh = WinBasedAttention(32, 4, 8, rotary=10000.0).rotary_plan("cpu")
+    assert torch.equal(blk.rotary_plan("cpu").table, fresh.table) and not torch.equal(fresh.table, first.table)
+    blk.num_heads = 2
+    assert blk.rotary_plan("cpu").head_dim == 16
+    blk.num_heads, blk.rotary = 4, 100.0
+    assert blk.rotary_plan("cpu") is first
+    blk.rotary = -1.0
+    with pytest.raises(ValueError, match="base has to be positive"):
+        blk.rotary_plan("cpu")
