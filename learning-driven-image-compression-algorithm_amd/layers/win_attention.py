@@ -72,6 +72,8 @@ class WinBasedAttention(nn.Module):
     head's channel pairs each; windows see relative positions only, so the map's coordinates serve shifted windows
     too.  Parameters and state_dict keys stay those of the block without it (the bias table is still added)."""
 
+    rotary: Optional[float] = None   # of blocks stored whole before they had it
+
     def __init__(self, dim=192, num_heads=8, window_size=8, shift_size=0, qkv_bias=True, qk_scale=None, drop=0.,
                  attn_drop=0., drop_path=0., rotary: Optional[float] = None):
         super().__init__()

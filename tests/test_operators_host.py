@@ -355,3 +355,11 @@ def test_rotary_plan_follows_the_block():
     blk.rotary = -1.0
     with pytest.raises(ValueError, match="base has to be positive"):
         blk.rotary_plan("cpu")
+
+
+def test_block_stored_whole_before_it_had_rotary():
+    """A block pickled as a module when the attribute did not exist runs as one without rotary positions."""
+    from lic_amd.layers import WinBasedAttention
+    blk = WinBasedAttention(32, 4, 8)
+    del blk.__dict__["rotary"]
+    assert blk.rotary is None
