@@ -70,7 +70,8 @@ class WindowAttention(nn.Module):
 class WinBasedAttention(nn.Module):
     """``rotary``: a base (e.g. 100.0) turns q and k by their token's row and column before the scores, half of a
     head's channel pairs each; windows see relative positions only, so the map's coordinates serve shifted windows
-    too.  Parameters and state_dict keys stay those of the block without it (the bias table is still added)."""
+    too.  Parameters and state_dict keys stay those of the block without it (the bias table is still added); the base is
+    in the state's metadata, and a state trained with another one is refused as one with an unexpected key is."""
 
     rotary: Optional[float] = None   # of blocks stored whole before they had it
 
@@ -87,6 +88,19 @@ class WinBasedAttention(nn.Module):
         assert 0 <= self.shift_size < self.window_size, "shift_size must in 0-window_size"
         self.attn = WindowAttention(dim, window_size=(window_size, window_size), num_heads=num_heads,
                                     qkv_bias=qkv_bias, qk_scale=qk_scale, attn_drop=attn_drop, proj_drop=drop)
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        if self.rotary is not None and hasattr(destination, "_metadata"):
+            destination._metadata.setdefault(prefix[:-1], {})["rotary"] = float(self.rotary)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                              error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                                      error_msgs)
+        base = local_metadata.get("rotary")
+        if base is not None and base != self.rotary:
+            unexpected_keys.append(f"{prefix}rotary (base {base} in the state, {self.rotary} here)")
 
     def rotary_plan(self, device) -> Fn.RotaryPlan:
         """The q / k rotation's plan on a device (kept for what it is made of: it holds only constants)."""

@@ -363,3 +363,32 @@ def test_block_stored_whole_before_it_had_rotary():
     blk = WinBasedAttention(32, 4, 8)
     del blk.__dict__["rotary"]
     assert blk.rotary is None
+
+
+def test_rotary_base_travels_with_a_state():
+    """The keys are those of a block without rotary positions, so the base is in the state's metadata: a strict load into a
+    block of another base, or of none, is refused, also through a file.  A load that is not strict goes through and says so;
+    so does a state that names no base: a block without one (whose weights may be turned from then on), another program's."""
+    import collections
+    import io
+    from lic_amd.layers import WinBasedAttention, Win_noShift_Attention
+    plain, turned, other = (WinBasedAttention(32, 4, 8, rotary=r) for r in (None, 100.0, 10000.0))
+    file = io.BytesIO()
+    torch.save(turned.state_dict(), file)
+    file.seek(0)
+    stored = torch.load(file, weights_only=True)
+    for state in (turned.state_dict(), stored):
+        with pytest.raises(RuntimeError, match="rotary"):
+            plain.load_state_dict(state)
+        with pytest.raises(RuntimeError, match="rotary"):
+            other.load_state_dict(state)
+        WinBasedAttention(32, 4, 8, rotary=100.0).load_state_dict(state)
+        assert "rotary" in plain.load_state_dict(state, strict=False).unexpected_keys[0]
+        plain.load_state_dict(collections.OrderedDict(state.items()))   # no metadata: other programs' files
+    turned.load_state_dict(plain.state_dict())
+    WinBasedAttention(32, 4, 8).load_state_dict(plain.state_dict())
+    # nested blocks, named by their place
+    a, b = Win_noShift_Attention(32, 4, 8, 4, rotary=100.0), Win_noShift_Attention(32, 4, 8, 4)
+    with pytest.raises(RuntimeError, match=r"conv_b\.0.*rotary"):
+        b.load_state_dict(a.state_dict())
+    b.load_state_dict(Win_noShift_Attention(32, 4, 8, 4).state_dict())
