@@ -1297,9 +1297,9 @@ def int8_mode() -> bool:
 
 
 class int8_linears:
-    """Context: layers.Linear (the qkv and proj products of the window-attention blocks) runs on linear_int8, weights
-    quantised once per parameter version.  Thread-local, forward only.  Encoder and decoder have to agree on it, as on
-    the precision."""
+    """Context: the layers.Linear with ``int8`` set (the qkv and proj products of the window-attention blocks, no others
+    unless a program sets it) run on linear_int8, weights quantised once per parameter version.  Thread-local, forward only.
+    Encoder and decoder have to agree on it, as on the precision."""
 
     def __init__(self, on: bool = True):
         self.on = bool(on)

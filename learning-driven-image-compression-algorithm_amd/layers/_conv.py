@@ -92,7 +92,10 @@ class Conv2d(nn.Conv2d, _PackCache):
 
 
 class Linear(nn.Linear, _PackCache):
-    """nn.Linear applied per pixel of an NHWC map (a 1x1 convolution)."""
+    """nn.Linear applied per pixel of an NHWC map (a 1x1 convolution).  ``int8``: whether functional.int8_linears takes
+    this layer (the window-attention blocks' qkv and proj are taken)."""
+
+    int8 = False
 
     def packed(self, dtype: torch.dtype) -> Fn.ConvPack:
         return self._get_pack(dtype, lambda: Fn.pack_conv2d(self.weight[:, :, None, None], self.bias, 1,
@@ -102,9 +105,9 @@ class Linear(nn.Linear, _PackCache):
         return self._get_pack("int8", lambda: Fn.pack_linear_int8(self.weight, self.bias))
 
     def run(self, x: Act, out: Optional[Act] = None, **kw) -> Act:
-        """Inside functional.int8_linears the product runs in 8-bit integers, for the epilogues linear_int8 has
-        (activation and residual); other calls keep the activation dtype's products."""
-        if Fn.int8_mode() and kw.keys() <= {"act", "slope", "r1"} and kw.get("act", ACT_NONE) != ACT_ROUND:
+        """Inside functional.int8_linears the product of a layer with ``int8`` runs in 8-bit integers, for the epilogues
+        linear_int8 has (activation and residual); other calls keep the activation dtype's products."""
+        if self.int8 and Fn.int8_mode() and kw.keys() <= {"act", "slope", "r1"} and kw.get("act", ACT_NONE) != ACT_ROUND:
             return Fn.linear_int8(x, self.packed_int8(), out, **kw)
         return Fn.conv(x, self.packed(x.dtype), out, **kw)
 

@@ -64,6 +64,7 @@ class WindowAttention(nn.Module):
         self.register_buffer("relative_position_index", rel.sum(-1))
         self.qkv = Linear(dim, dim * 3, bias=qkv_bias)
         self.proj = Linear(dim, dim)
+        self.qkv.int8 = self.proj.int8 = True   # taken by functional.int8_linears
         _trunc_normal_(self.relative_position_bias_table, std=.02)
 
 
@@ -119,7 +120,7 @@ class WinBasedAttention(nn.Module):
         (bit-identical, but slower today: DESIGN.md section 5)."""
         # rotary positions go between the qkv product and the scores, 8-bit Linears replace the product: both
         # take the three-launch path
-        plain = self.rotary is None and not Fn.int8_mode()
+        plain = self.rotary is None and not (Fn.int8_mode() and (self.attn.qkv.int8 or self.attn.proj.int8))
         if plain and _FUSED and Fn.wba_qkv_attn_ok(x, self.dim, self.num_heads, self.window_size):
             # the fused proj stores 16 B per lane: only into a fresh buffer or a 16-B aligned view
             # with 4-element rows, never onto x (the shortcut) -- else the proj runs as its own launch

@@ -392,3 +392,32 @@ def test_rotary_base_travels_with_a_state():
     with pytest.raises(RuntimeError, match=r"conv_b\.0.*rotary"):
         b.load_state_dict(a.state_dict())
     b.load_state_dict(Win_noShift_Attention(32, 4, 8, 4).state_dict())
+
+
+def test_int8_linears_scope(monkeypatch):
+    """Inside the context the window-attention blocks' qkv and proj products run in 8 bits and no other Linear: not the
+    generator of the decoder's filters, nor the entropy parameters' blocks and MLPs.  A layer of one's own opts in."""
+    import bench
+    from lic_amd.layers import Linear, WinBasedAttention
+    net = bench.build_net("net_ga", "fp16", 256, 1, "cpu")
+    blocks = {n for n, m in net.named_modules() if isinstance(m, WinBasedAttention)}
+    linears = {n: m for n, m in net.named_modules() if isinstance(m, Linear)}
+    inside = {n for b in blocks for n in (b + ".attn.qkv", b + ".attn.proj")}
+    assert inside < linears.keys()
+    seen = []
+    monkeypatch.setattr(Linear, "packed", lambda self, dtype: None)
+    monkeypatch.setattr(Linear, "packed_int8", lambda self: None)
+    monkeypatch.setattr(Fn, "conv", lambda *a, **k: None)
+    monkeypatch.setattr(Fn, "linear_int8", lambda *a, **k: seen.append(True))
+
+    def eighth(m):
+        seen.clear()
+        m.run(Act(torch.zeros(1, 1, 1, m.in_features)))
+        return bool(seen)
+    assert not any(eighth(m) for m in linears.values())
+    with Fn.int8_linears():
+        assert {n for n, m in linears.items() if eighth(m)} == inside
+        own = Linear(16, 16)
+        assert not eighth(own)
+        own.int8 = True
+        assert eighth(own)
