@@ -94,14 +94,18 @@ class Muon(torch.optim.Optimizer):
             orth = Fn.orthogonalize(mats, steps=group["steps"], eps=group["eps"])
             orth = [o.view(p.shape) for o, p in zip(orth, params)]   # fp32: only the new weight is rounded to its type
             torch._foreach_mul_(orth, [self._scale(group["adjust"], *m.shape) for m in mats])
+            if wd:
+                # weights of other types: the decay joins the fp32 update, a multiply of its own would round it away
+                exact = [p for p in params if p.dtype == torch.float32]
+                if exact:
+                    torch._foreach_mul_(exact, 1.0 - lr * wd)
+                for p, o in zip(params, orth):
+                    if p.dtype != torch.float32:
+                        o.add_(p.float(), alpha=wd)
             if isinstance(lr, torch.Tensor):
                 torch._foreach_mul_(orth, lr)
-                if wd:
-                    torch._foreach_mul_(params, 1.0 - lr * wd)
                 torch._foreach_sub_(params, orth)
             else:
-                if wd:
-                    torch._foreach_mul_(params, 1.0 - lr * wd)
                 torch._foreach_sub_(params, orth, alpha=lr)
         return loss
 

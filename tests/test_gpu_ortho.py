@@ -245,3 +245,23 @@ def test_train_cli_with_muon(mode, monkeypatch, capsys):
     out = capsys.readouterr().out
     loss = float(re.search(r"\[Epoch 0000 TRAIN\] Loss: (\S+)", out).group(1))
     assert math.isfinite(loss) and loss > 0
+
+
+@pytest.mark.parametrize("wd", [0.05, 2.0])
+def test_muon_16_bit_decay(wd):
+    """bf16 weights, decay and update are rounded together, once: also a decay (lr wd = 5e-4 of the weight) that a bf16
+    multiply would lose (half a step is 2^-8).  Tolerance: half a step of the result, and the update's own error, 1e-5 of
+    its norm at most (4 * 2.5e-6)."""
+    from lic_amd.optim import Muon
+    g = torch.Generator().manual_seed(10)
+    w, grad = torch.randn(40, 64, generator=g).bfloat16(), torch.randn(40, 64, generator=g).bfloat16()
+    x = _newton_schulz(grad.double(), 5, C, 1e-7, torch.float64)
+    for lr in (0.01, torch.tensor(0.01, device=DEV)):
+        p = torch.nn.Parameter(w.to(DEV))
+        p.grad = grad.to(DEV)
+        Muon([p], lr=lr, momentum=0.0, adjust="shape", weight_decay=wd).step()
+        want = w.double() * (1 - 0.01 * wd) - 0.01 * x
+        tol = torch.finfo(torch.bfloat16).eps / 2 * want.abs() + 0.01 * 1e-5 * math.sqrt(40)
+        assert ((p.detach().cpu().double() - want).abs() <= tol).all()
+        lost = (w.double() - 0.01 * x).bfloat16()
+        assert not torch.equal(p.detach().cpu(), lost)

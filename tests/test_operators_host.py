@@ -421,3 +421,37 @@ def test_int8_linears_scope(monkeypatch):
         assert not eighth(own)
         own.int8 = True
         assert eighth(own)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tensor_lr", [False, True])
+@pytest.mark.parametrize("wd", [0.01, 1.0, 30.0])
+def test_muon_decay_rounds_with_the_update(monkeypatch, dtype, tensor_lr, wd):
+    """w <- w - (lr scale X + lr wd w) rounded once to w's type, decays far below its step included (lr wd 1e-5 of w here
+    at the least, a bf16 step is 2^-7 of it).  X is given here in multiples that put w - update next to borders.
+    Tolerance: half a step of the result, and the update's few fp32 roundings, 4 * 2^-24 of its terms; for fp32 weights, whose
+    decay is a product of its own, three roundings of the weight."""
+    from lic_amd.optim import Muon
+    g = torch.Generator().manual_seed(3)
+    w, x = torch.randn(16, 24, generator=g).to(dtype), torch.randn(16, 24, generator=g)
+    # with this, lr * 0.2 sqrt(24) * x is an odd number of half steps of w, and the decay decides
+    step = torch.finfo(dtype).eps * torch.exp2(torch.floor(torch.log2(w.float().abs())))
+    lr, scale = 1e-3, 0.2 * math.sqrt(24)
+    x[::2] = (step * 0.5 / (lr * scale))[::2] * torch.sign(w.float()[::2])
+    monkeypatch.setattr(Fn, "orthogonalize", lambda mats, **k: [x.clone() for _ in mats])
+    monkeypatch.setattr(Fn, "_on_current_device", lambda *a: None)
+    p = torch.nn.Parameter(w.clone())
+    p.grad = torch.ones_like(p)
+    Muon([p], lr=torch.tensor(lr) if tensor_lr else lr, weight_decay=wd).step()
+    lr64 = float(torch.tensor(lr)) if tensor_lr else lr
+    upd, decay = lr64 * scale * x.double(), lr64 * wd * w.double()
+    want = w.double() - upd - decay
+    eps = torch.finfo(dtype).eps
+    tol = eps / 2 * want.abs() + 4 * 2.0 ** -24 * (upd.abs() + decay.abs())
+    if dtype == torch.float32:
+        tol = tol + eps * w.double().abs()
+    assert ((p.detach().double() - want).abs() <= tol).all()
+    assert p.dtype == dtype
+    if dtype != torch.float32:   # the decay is there: without it, the even rows' ties would round elsewhere
+        off = (p.detach() != (w.double() - upd).to(dtype)).double().mean()
+        assert off > 0.05
