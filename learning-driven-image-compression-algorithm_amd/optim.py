@@ -80,12 +80,13 @@ class Muon(torch.optim.Optimizer):
                 continue
             Fn._on_current_device("Muon", *params)
             lr, mu, wd = group["lr"], group["momentum"], group["weight_decay"]
-            bufs = []
-            for p in params:
-                st = self.state[p]
-                if "momentum" not in st:
-                    st["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-                bufs.append(st["momentum"])
+            new = [p for p in params if "momentum" not in self.state[p]]
+            if new and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Muon: capture after one eager step of these parameters (a graph that creates their "
+                                   "momentum would set it to zero at every replay)")
+            for p in new:
+                self.state[p]["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            bufs = [self.state[p]["momentum"] for p in params]
             grads = [p.grad.float() for p in params]
             # m <- mu m + (1 - mu) g;  u = mu m + (1 - mu) g (Nesterov) or m
             torch._foreach_lerp_(bufs, grads, 1.0 - mu)

@@ -265,3 +265,19 @@ def test_muon_16_bit_decay(wd):
         assert ((p.detach().cpu().double() - want).abs() <= tol).all()
         lost = (w.double() - 0.01 * x).bfloat16()
         assert not torch.equal(p.detach().cpu(), lost)
+
+
+def test_muon_captured_without_a_step_before_is_refused():
+    """A graph that created the momentum would set it to zero at every replay."""
+    from lic_amd.optim import Muon
+    p = torch.nn.Parameter(torch.randn(16, 16, device=DEV))
+    p.grad = torch.randn_like(p)
+    opt, before, graph = Muon([p], lr=torch.tensor(0.01, device=DEV)), p.detach().clone(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="eager step"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(p, before) and not opt.state[p]
+    opt.step()
+    assert not torch.equal(p, before) and "momentum" in opt.state[p]

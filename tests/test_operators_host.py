@@ -455,3 +455,22 @@ def test_muon_decay_rounds_with_the_update(monkeypatch, dtype, tensor_lr, wd):
     if dtype != torch.float32:   # the decay is there: without it, the even rows' ties would round elsewhere
         off = (p.detach() != (w.double() - upd).to(dtype)).double().mean()
         assert off > 0.05
+
+
+def test_muon_captured_without_a_step_before_is_refused(monkeypatch):
+    """A graph that created the momentum would set it to zero at every replay."""
+    from lic_amd.optim import Muon
+    monkeypatch.setattr(Fn, "orthogonalize", lambda mats, **k: [m.clone() for m in mats])
+    monkeypatch.setattr(Fn, "_on_current_device", lambda *a: None)
+    p = torch.nn.Parameter(torch.ones(8, 8))
+    p.grad = torch.ones(8, 8)
+    opt = Muon([p], lr=0.5)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="eager step"):
+        opt.step()
+    assert torch.equal(p, torch.ones(8, 8)) and not opt.state[p]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    opt.step()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    opt.step()
