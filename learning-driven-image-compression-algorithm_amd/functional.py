@@ -1080,6 +1080,12 @@ def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
             raise ValueError(f"{what}: tensor on {t.device}, the current device is cuda:{dev}")
 
 
+def _in_32_bits(what: str, *sizes: int) -> None:
+    """The C entries' sizes have 32 bits, and ctypes cuts longer ones off without a word."""
+    if max(sizes) >= 1 << 31:
+        raise ValueError(f"{what}: sizes of 2^31 and more are out of range")
+
+
 def _overlaps(a: Act, b: Act) -> bool:
     """Whether two views can share an element (channel windows of one tensor are told apart)."""
     if not a.t.numel() or a.t.untyped_storage().data_ptr() != b.t.untyped_storage().data_ptr():
@@ -1147,6 +1153,7 @@ def rotary(x: Act, plan: RotaryPlan, heads: int, positions: Optional[torch.Tenso
     c, dtype = x.c, x.t.dtype
     if heads < 1 or heads * plan.head_dim > c:
         raise ValueError(f"rotary: {heads} heads of {plan.head_dim} channels do not fit a view of {c}")
+    _in_32_bits("rotary", B * H * W, ld, ld if out is None else out.ld)
     _on_current_device("rotary", x.t, plan.table, positions)
     pos_ptr, per_image = None, 0
     if positions is not None:
@@ -1221,6 +1228,7 @@ def _quantize_int8(x_ptr: int, ldx: int, dtype: torch.dtype, m: int, k: int, dev
 def quantize_tokens(x: Act) -> Int8Act:
     """One scale per token, max|x| / 127, and codes rint(127 x / max|x|) (exact, half to even).  A token that holds a
     NaN or an infinity gets a NaN scale.  For several linear_int8 calls on one map."""
+    _in_32_bits("quantize_tokens", x.npix)
     _on_current_device("quantize_tokens", x.t)
     if not 1 <= x.c <= INT8_MAX_K:
         raise ValueError(f"quantize_tokens: 1 to {INT8_MAX_K} channels, got {x.c}")
@@ -1235,6 +1243,7 @@ def pack_linear_int8(weight: torch.Tensor, bias: Optional[torch.Tensor] = None) 
                          f"{tuple(weight.shape)}")
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise ValueError("pack_linear_int8: bias must be [co]")
+    _in_32_bits("pack_linear_int8", weight.shape[0])
     _on_current_device("pack_linear_int8", weight, bias)
     w = weight.detach().contiguous()
     codes, scale = _quantize_int8(_dp(w), w.shape[1], w.dtype, w.shape[0], w.shape[1], w.device)
@@ -1258,6 +1267,7 @@ def linear_int8(x, pk: Int8Pack, out: Optional[Act] = None, *, act: int = _ffi.A
     dtype, co, r1t = x.dtype, pk.w.shape[0], r1.t if r1 is not None else None
     if x.c != pk.ci:
         raise ValueError(f"linear_int8: input has {x.c} channels, weights expect {pk.ci}")
+    _in_32_bits("linear_int8", B * H * W, co)
     _on_current_device("linear_int8", src, pk.w, r1t)
     if act not in _INT8_ACTS:
         raise ValueError("linear_int8: act must be ACT_NONE, ACT_RELU, ACT_LRELU or ACT_GELU")
@@ -1333,6 +1343,7 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs: Sequence
     for g in mats:
         if g.dim() != 2 or g.dtype != dt:
             raise ValueError("orthogonalize: a list of 2-D matrices of one dtype")
+    _in_32_bits("orthogonalize", *(n for g in mats for n in g.shape))
     _on_current_device("orthogonalize", *mats)
     if len(coeffs) != 3 or not all(math.isfinite(c) for c in coeffs):
         raise ValueError("orthogonalize: coeffs = (a, b, c), finite")

@@ -474,3 +474,29 @@ def test_muon_captured_without_a_step_before_is_refused(monkeypatch):
     opt.step()
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     opt.step()
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """The C entries take 32-bit sizes, and a call by ctypes cuts longer ones off: 2^32 + 1 tokens would be one."""
+    def meta(*shape, dtype=torch.float16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+    long = Act(meta(1, 2, 2 ** 31 + 1, 2))
+    pk = Fn.Int8Pack(meta(4, 64, dtype=torch.int8), meta(4, dtype=torch.float32), None, 2)
+    q = Fn.Int8Act(meta(1, 2, 2 ** 31 + 1, 64, dtype=torch.int8), meta(1, 2, 2 ** 31 + 1, dtype=torch.float32), 2,
+                   torch.float16)
+    with pytest.raises(ValueError, match="out of range"):
+        Fn.rotary(long, _plan(2, (1,)), 1)
+    with pytest.raises(ValueError, match="out of range"):
+        Fn.rotary(Act(meta(1, 1, 1, 2 ** 32 + 64), 0, 2), _plan(2, (1,)), 1)
+    with pytest.raises(ValueError, match="out of range"):
+        Fn.rotary(Act(meta(1, 1, 1, 2)), _plan(2, (1,)), 1, out=Act(meta(1, 1, 1, 2 ** 32 + 64), 0, 2))
+    for x in (long, q):
+        with pytest.raises(ValueError, match="out of range"):
+            Fn.linear_int8(x, pk)
+    with pytest.raises(ValueError, match="out of range"):
+        Fn.quantize_tokens(long)
+    with pytest.raises(ValueError, match="out of range"):
+        Fn.pack_linear_int8(meta(2 ** 32 + 1, 2))
+    for shape in ((2 ** 32 + 1, 2), (2, 2 ** 32 + 1)):
+        with pytest.raises(ValueError, match="out of range"):
+            Fn.orthogonalize([meta(*shape)])
