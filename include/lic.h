@@ -618,7 +618,8 @@ int lic_rotary(int32_t dtype, const void* x, int32_t ldx, int32_t n, int32_t h, 
  * Either xcodes / xscale ([m][kpad], fp32 [m]) or x (m rows of k, stride ldx, quantised by the call) is given.
  * act: LIC_ACT_NONE / RELU / LRELU / GELU; bias and r1 may be NULL; y must not overlap x, xcodes or w (r1 may
  * be y).  ws: with x, lic_linear_int8_workspace bytes, 16-byte aligned (0: small calls need none).  x, y, r1, wscale and
- * bias may lie at any multiple of their elements' size. */
+ * bias may lie at any multiple of their elements' size.  Up to 2^31 - 256 tokens, 2^27 - 16 channels and less than 2^24
+ * tiles of 128 x 128 in y.  xscale[i] * wscale[o] is formed first and has to be a finite fp32 number. */
 #define LIC_INT8_MAX_K 131072
 int lic_quantize_int8(int32_t dtype, const void* x, int64_t ldx, int32_t m, int32_t k, int8_t* codes, int32_t kpad,
                       float* scale, lic_stream_t stream);
@@ -636,7 +637,7 @@ int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const int8_t* xco
  * gives zeros, one with a NaN or an infinity nothing finite.  Deterministic (no atomics); a matrix's result
  * does not depend on its neighbours in the list.
  * ws: lic_orthogonalize_workspace bytes of device memory, 256-byte aligned, -1: sizes out of range (a shorter
- * side above 65536, a longer one above 2^24, more than 2^30 tiles of 64 x 64 in all). */
+ * side above 65536, a longer one above 2^24, 2^24 tiles of 64 x 64 and more in all). */
 typedef struct lic_ortho_mat {
   const void* g; int64_t rs, cs;
   void* out;

@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void quantize_int8_kernel(const T* __restrict_
   constexpr int V = QUANT_V<T>;
   constexpr int NV = 4;
   const int lane = threadIdx.x & (G - 1);
-  const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (256 / G) + threadIdx.x / G;
   if (row >= m) return;
   const T* xr = x + row * ldx;
   QuantVec<T, V> v[NV];
@@ -804,8 +804,10 @@ static int quantize_run(const void* x, int64_t ldx, int m, int k, int8_t* codes,
                         hipStream_t s) {
   const int vecs = kpad / QUANT_V<T>;
   auto launch = [&](auto kernel, int rows) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)m + rows - 1) / rows)), dim3(256), 0, s, (const T*)x, ldx, m, k,
-                       codes, kpad, scale);
+    // a dimension of a launch has less than 2^32 threads
+    const int64_t blocks = ((int64_t)m + rows - 1) / rows, bx = std::min<int64_t>(blocks, 1 << 22);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)bx, (unsigned)((blocks + bx - 1) / bx)), dim3(256), 0, s, (const T*)x, ldx, m,
+                       k, codes, kpad, scale);
   };
   if (vecs <= 32 && m > QUANT_FEW) launch(quantize_int8_kernel<T, 8>, 32);
   else if (vecs <= 64 && m > QUANT_FEW) launch(quantize_int8_kernel<T, 16>, 16);
@@ -824,7 +826,6 @@ static int quantize_any(int32_t dtype, const void* x, int64_t ldx, int m, int k,
 template <typename T, int BM, int BN, int WM, int WN, int KG>
 static int tile_launch(const Int8Args& a, hipStream_t s) {
   const int mt = (int)(((int64_t)a.m + BM - 1) / BM), nt = (a.n + BN - 1) / BN;
-  if ((int64_t)mt * nt > INT32_MAX / 8) return fail("linear_int8: m x n out of range");
   constexpr int LDS = KG * 4 * (BM + BN) * 64;
   const void* k = (const void*)int8_tile_kernel<T, BM, BN, WM, WN, KG>;
   if (ensure_dyn_lds(k, LDS) != hipSuccess) return fail("linear_int8: LDS limit");
@@ -928,7 +929,10 @@ extern "C" int lic_linear_int8(int32_t dtype, const void* x, int64_t ldx, const 
                                void* y, int64_t ldy, void* ws, int64_t ws_bytes, lic_stream_t stream) {
   using namespace lic;
   if (check_sizes("linear_int8", dtype, m, k, kpad)) return 1;
-  if (n < 1 || n > (1 << 30)) return fail("linear_int8: n out of range");
+  // a launch has less than 2^32 threads: 256 for a tile of 128 x 128 or 128 tokens, 512 for one of 256 x 256 or 16 channels
+  if (m > INT32_MAX - 255) return fail("linear_int8: m out of range");
+  if (n < 1 || n > (1 << 27) - 16) return fail("linear_int8: n out of range");
+  if (((int64_t)m + 127) / 128 * (((int64_t)n + 127) / 128) >= 1 << 24) return fail("linear_int8: m x n out of range");
   if (act < LIC_ACT_NONE || act > LIC_ACT_GELU) return fail("linear_int8: act has to be none, relu, lrelu or gelu");
   if (m == 0) return 0;
   if (!w || !wscale || !y || ldy < n || (r1 && ldr1 < n)) return fail("linear_int8: null pointer or row stride below n");

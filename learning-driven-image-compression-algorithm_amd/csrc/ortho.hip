@@ -548,7 +548,6 @@ static bool ortho_plan(int count, const lic_ortho_mat* mats, OrthoPlan& p, Ortho
     const int64_t r = flip ? m.cols : m.rows, c = flip ? m.rows : m.cols;
     if (r < 1 || r > 65536 || c > (1 << 24)) return false;
     const int64_t nr = up(r, 64) / 64, nc = up(c, 64) / 64, x = nr * nc * 8192, a = nr * nr * 8192;   // halves, both parts
-    if (nr * nc > (1 << 28)) return false;
     OrthoDesc o{m.g, m.out, flip ? m.cs : m.rs, flip ? m.rs : m.cs};
     o.r = (int32_t)r;
     o.c = (int32_t)c;
@@ -578,7 +577,8 @@ static bool ortho_plan(int count, const lic_ortho_mat* mats, OrthoPlan& p, Ortho
     p.parts += nr * nc;
     p.gram += lower;
     p.upd += nr * ((nc + 3) / 4);
-    if (p.parts > (1 << 30) || p.slices > (1 << 30) || p.upd > (1 << 30)) return false;
+    // a launch of workgroups of 256 has less than 2^32 threads
+    if (p.parts >= 1 << 24 || p.slices >= 1 << 24 || p.upd >= 1 << 24) return false;
     if (d) d[i] = o;
   }
   p.count += count;

@@ -70,7 +70,9 @@ template <typename T, int V, bool HALF, RotaryForm FORM>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   extern __shared__ float2 turn[];   // [tokens of the block][pairs]
   typedef T Vec __attribute__((ext_vector_type(V)));
-  const int t0 = (int)blockIdx.x * a.per_block;
+  const int64_t first = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.per_block;
+  if (first >= a.tokens) return;
+  const int t0 = (int)first;
   const int nt = min(a.per_block, a.tokens - t0);
   for (int i = threadIdx.x; i < nt * a.pairs; i += 256) {
     const int t = rotary_div(i, a.inv_pairs), p = i - t * a.pairs;
@@ -161,9 +163,11 @@ static int rotary_launch(RotaryArgs a, hipStream_t s) {
   a.inv_vecs = a.per_block > 1 ? rotary_inverse(a.vecs) : 1;
   a.inv_head_vecs = rotary_inverse(a.head_vecs);
   a.inv_pairs = rotary_inverse(a.pairs);
+  // a dimension of a launch has less than 2^32 threads
   const unsigned blocks = (unsigned)(((int64_t)a.tokens + a.per_block - 1) / a.per_block);
+  const unsigned bx = blocks < 1u << 22 ? blocks : 1u << 22;
   const unsigned lds = (unsigned)(a.per_block * a.pairs * sizeof(float2));
-  hipLaunchKernelGGL((rotary_kernel<T, V, HALF, FORM>), dim3(blocks), dim3(256), lds, s, a);
+  hipLaunchKernelGGL((rotary_kernel<T, V, HALF, FORM>), dim3(bx, (blocks + bx - 1) / bx), dim3(256), lds, s, a);
   LIC_CHECK_LAUNCH();
   return 0;
 }

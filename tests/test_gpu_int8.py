@@ -298,3 +298,25 @@ def test_linear_int8_streams_and_graph():
         torch.cuda.synchronize()
         for x, o in zip(xs, outs):
             assert torch.equal(o, Fn.linear_int8(Fn.Act(x), pk).t)
+
+
+def test_codes_of_more_workgroups_than_a_grid_dimension():
+    """From 2^26 rows of more than 512 channels on (four a workgroup of 256 threads) a launch takes a second dimension:
+    rows on both sides of its own, zeros everywhere else (69 GB of rows)."""
+    import lic_amd.functional as Fn
+    m, k = (1 << 26) + 5, 513
+    at = torch.tensor([0, 3, 4, (1 << 24) - 1, 1 << 24, (1 << 26) - 1, 1 << 26, m - 2, m - 1], device=DEV)
+    x = torch.zeros(1, 1, m, k, dtype=torch.bfloat16, device=DEV)
+    rows = torch.randn(at.numel(), k, generator=torch.Generator().manual_seed(2)).bfloat16()
+    x.view(m, k)[at] = rows.to(DEV)
+    q = Fn.quantize_tokens(Fn.Act(x))
+    codes, scale = q.codes.view(m, -1), q.scale.view(m)
+    got, gots = codes[at].cpu(), scale[at].cpu()
+    codes[at], scale[at] = 0, 0
+    assert all(int(torch.count_nonzero(part)) == 0 for part in codes.split(1 << 21))
+    assert int(torch.count_nonzero(scale)) == 0
+    del x, q, codes, scale
+    torch.cuda.empty_cache()
+    want, wants = _codes(rows)
+    assert torch.equal(got[:, :k].double(), want) and (got[:, k:] == 0).all()
+    assert ((gots.double() - wants).abs() <= U * wants).all()

@@ -224,3 +224,24 @@ def test_rotary_other_stream_and_graph():
         assert torch.equal(y, Fn.rotary(Fn.Act(sx.detach()), plan, 16).t)
         assert torch.equal(dx, Fn.rotary(Fn.Act(sg), plan, 16, inverse=True).t)
         assert torch.equal(z.t, Fn.rotary(Fn.Act(y.detach()), plan, 16, inverse=True).t)
+
+
+def test_rotary_more_workgroups_than_a_grid_dimension():
+    """From 2^24 workgroups of 256 threads on (here one token each: rows of 1025 elements are read one by one) a launch
+    takes a second dimension: tokens on both sides of its rows, zeros everywhere else (34 GB each way)."""
+    import lic_amd.functional as Fn
+    H = W = 4100
+    assert H * W > 1 << 24
+    plan = Fn.RotaryPlan(1025, (200, 312), device=DEV)
+    at = torch.tensor([0, 1, (1 << 22) - 1, 1 << 22, (1 << 22) + 1, (1 << 24) - 1, 1 << 24, H * W - 1])
+    x = torch.zeros(1, H, W, 1025, dtype=torch.bfloat16, device=DEV)
+    rows = torch.randn(at.numel(), 1025, generator=torch.Generator().manual_seed(2)).bfloat16()
+    x.view(H * W, 1025)[at.to(DEV)] = rows.to(DEV)
+    y = Fn.rotary(Fn.Act(x), plan, 1).t.view(H * W, 1025)
+    got = y[at.to(DEV)].clone()
+    y[at.to(DEV)] = 0
+    assert all(int(torch.count_nonzero(part)) == 0 for part in y.split(1 << 20))
+    del x, y
+    torch.cuda.empty_cache()
+    pos = torch.stack([at // W, at % W])[:, None, None]
+    _check(got.view(1, 1, -1, 1025), *_oracle(rows.view(1, 1, -1, 1025), plan, 1, pos))

@@ -500,3 +500,25 @@ def test_sizes_beyond_32_bits_are_refused():
     for shape in ((2 ** 32 + 1, 2), (2, 2 ** 32 + 1)):
         with pytest.raises(ValueError, match="out of range"):
             Fn.orthogonalize([meta(*shape)])
+
+
+def test_c_entries_refuse_what_no_launch_takes():
+    """A launch has less than 2^32 threads: products and lists of matrices beyond that are refused before anything runs."""
+    lib = lic_amd.load_library()
+    f = 4096
+
+    def lin(m, n, kpad=128):
+        return lib.lic_linear_int8(0, None, 0, f, f, m, 100, f, kpad, f, None, n, 0, 0.0, None, 0, f, n, None, 0, None)
+    _refused(lin(2 ** 31 - 255, 8), "m out of range")
+    _refused(lin(2 ** 31 - 1, 8), "m out of range")
+    _refused(lin(8, 2 ** 27 - 15), "n out of range")
+    _refused(lin(2 ** 30, 257), "m x n out of range")
+    _refused(lin(2 ** 20, 2 ** 19), "m x n out of range")
+
+    def tiles(rows, cols, count=1):
+        m = (_ffi.OrthoMat * count)()
+        for d in m:
+            d.g, d.rs, d.cs, d.out, d.rows, d.cols = f, cols, 1, f, rows, cols
+        return lib.lic_orthogonalize_workspace(0, count, m)
+    assert tiles(64, 2 ** 24) > 0 and tiles(64 * 63, 2 ** 24) > 0     # 63 * 2^18 tiles
+    assert tiles(64 * 64, 2 ** 24) == -1 and tiles(64, 2 ** 24, 64) == -1
