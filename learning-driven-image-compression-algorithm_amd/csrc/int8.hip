@@ -515,6 +515,7 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
   const int n0 = blockIdx.x * 16;
   const int steps = a.kpad / 64, s0 = steps * wave / 8, s1 = steps * (wave + 1) / 8;
   const int8_t* w = a.w + (int64_t)min(n0 + row, a.n - 1) * a.kpad + 16 * q;
+  static_assert(ONE_K <= 8 * 8 * 64, "a wave's steps of k are held at once");
   int32x4 fw[8];
 #pragma unroll
   for (int u = 0; u < 8; ++u)
@@ -560,9 +561,6 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
   for (int u = 0; u < 8; ++u)
     if (s0 + u < s1)
       acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], *(const int32x4*)(x + 64 * (s0 + u)), acc[0], 0, 0, 0);
-  for (int s = s0 + 8; s < s1; ++s)
-    acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const int32x4*)(w + 64 * s), *(const int32x4*)(x + 64 * s), acc[0],
-                                                   0, 0, 0);
   int8_join<T, 1>(a, part, acc, n0, 0, scale);
 }
 
