@@ -2,10 +2,14 @@
 //   X = G / (|G|_F + eps);  `steps` times: A = X X^T, X = (a I + b A + c A A) X
 // on r x c matrices with r <= c (G^T where G has more rows than columns).
 //
-// Every product runs on fp16 matrix instructions with operands of two parts, value = hi + lo (22 bits), as
-// hi hi' + hi lo' + lo hi' with fp32 sums: the error of fp32 products at three eighths of their cost (one part alone would
-// leave 4e-4 .. 3e-3 of the result, two parts leave what fp32 leaves, 2e-6 at 192 x 1728).  X is held divided by a power of
-// two above its norm (from |G| and the polynomial's bounds), so the parts never leave fp16's range.
+// Every product runs on fp16 matrix instructions with operands of two parts, value = hi + lo, as hi hi' + hi lo' + lo hi' with
+// fp32 sums.  So X, A and Q have 22 bits between the products, two less than fp32's: taken for its cost, three eighths of fp32
+// matrix instructions' (one part alone would leave 4e-4 .. 3e-3 of the result).  Error against 64 bits, over that of the same
+// iteration in fp32 products, in the Frobenius norm: 16 x 144 0.74, 64 x 64 1.01, 66 x 66 1.22, 128 x 128 1.15, 128 x 576
+// 1.12, 192 x 1728 1.03, 512 x 2304 0.79, 2048 x 2048 0.53 (3.0e-6 of the result for 5.6e-6).  More of it than of fp32's lies
+// along few directions: in the 2-norm 66 x 66 1.22, 192 x 1728 1.37, 512 x 2304 1.98, 2048 x 2048 2.11 (1.7e-5 for 8.1e-6).
+// X is held divided by a power of two above its norm (from |G| and the polynomial's bounds), so the parts never leave fp16's
+// range.
 //
 // Operands lie in fragment order: [row / 32][k / 16][hi, lo][64 lanes][8], one contiguous KB a fragment, loaded straight into
 // registers; place p of a 32-row tile is row 16 ((p / 4) % 2) + 4 (p / 8) + p % 4 of it.  With that order on both operands a
@@ -229,7 +233,7 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(OrthoWork w, OrthoBoun
 // 64 x 64 results of P R^T over k steps [s0, s1), operands in fragment order (two row tiles each): acc[i][j] is P's tile i
 // against R's tile j.
 // Steps that the matrix instructions sum up before the rounded fp32 addition to the total: their own additions of a long chain
-// lose more.  2-norm error at 2048 x 2048: one chain 8.9e-6, chains of 16 steps 4.0e-6, of 8 3.3e-6, of 4 3.0e-6 (fp32
+// lose more.  Error of the result (Frobenius) at 2048 x 2048: one chain 8.9e-6, chains of 16 steps 4.0e-6, of 8 3.3e-6, of 4 3.0e-6 (fp32
 // products: 5.6e-6); 128 x 576: 2.9e-6, .., 2.4e-6 (2.2e-6).  4 costs 1 to 3 % of the time.
 constexpr int ORTHO_CHAIN = 4;
 struct OrthoFrags { half8 p[2][2], r[2][2]; };
@@ -298,8 +302,8 @@ __device__ __forceinline__ void ortho_product(floatx16 (&sum)[2][2], const half_
 }
 
 // What two parts leave out of Q X, for matrices whose short sums would show it: Q's low part with X's, Q's high part with X's
-// third, which is what fp32 holds of X beyond 22 bits.  The error against 64 bits is mostly that of X between the steps; 2-norm
-// against that of fp32 products: 16 x 144 1.20 -> 0.81 of it, 64 x 64 1.25 -> 1.02; 66 x 66, without, 1.24, 128 x 128 1.13,
+// third, which is what fp32 holds of X beyond 22 bits.  The error against 64 bits is mostly that of X between the steps;
+// Frobenius norm against that of fp32 products: 16 x 144 1.20 -> 0.81 of it, 64 x 64 1.25 -> 1.02; 66 x 66, without, 1.24, 128 x 128 1.13,
 // 192 x 192 1.01, where the sums' own rounding is as large.  64 x 576 91.9 -> 103.3 us; up to 128 rows 128 x 576 would be 135.
 constexpr int ORTHO_FINE = 64;
 __device__ __forceinline__ void ortho_finer(floatx16 (&sum)[2][2], const half_t* x, const half_t* rest, const half_t* q,

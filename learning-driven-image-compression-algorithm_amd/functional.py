@@ -1335,7 +1335,8 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs: Sequence
     than columns).  Drives the singular values towards 1: the update direction of the Muon optimiser.
 
     Matrices: 2-D, of one dtype (fp32, fp16, bf16), any strides.  Returns contiguous matrices of that dtype; everything
-    in between is held in fp32 or in two fp16 parts (22 bits)."""
+    in between is held in fp32 or in two fp16 parts (22 bits), which leaves up to 1.25 times the error of fp32 products
+    (Frobenius norm; 2-norm: up to about 2.1 times)."""
     mats = list(mats)
     if not mats:
         return []

@@ -281,3 +281,39 @@ def test_muon_captured_without_a_step_before_is_refused():
     assert torch.equal(p, before) and not opt.state[p]
     opt.step()
     assert not torch.equal(p, before) and "momentum" in opt.state[p]
+
+
+# error against that of fp32 products, and the bound: midway between the recorded ratio and the one without what the shape
+# is there for (16 x 144, 64 x 64: the third part of X, 1.20 and 1.25 without; 128 x 576, 2048 x 2048: short chains of the
+# matrix instructions' own additions, 1.32 and 0.71 with chains of 16 steps)
+@pytest.mark.parametrize("m,n,bound", [(16, 144, (0.81 + 1.20) / 2), (64, 64, (1.02 + 1.25) / 2),
+                                       (128, 576, (1.09 + 1.32) / 2), (2048, 2048, (0.54 + 0.71) / 2)])
+def test_orthogonalize_error_against_fp32_products(m, n, bound):
+    """Frobenius norms, averaged over four seeds; fp32 products by the library's plain fp32 matrix product."""
+    import lic_amd.functional as Fn
+
+    def products(g, dt):
+        a, b, c = C
+        x = g.double()
+        x = (x / (torch.linalg.vector_norm(x) + 1e-7)).to(dt)
+        for _ in range(5):
+            gram = torch.mm(x, x.t().contiguous())
+            x = a * x + torch.mm(b * gram + c * torch.mm(gram, gram), x)
+        return x.double()
+    kernel = plain = 0.0
+    for seed in range(4):
+        g = _gradient(m, n, torch.Generator().manual_seed(20 + seed), torch.float32).to(DEV)
+        want = products(g, torch.float64)
+        kernel += float((Fn.orthogonalize([g])[0].double() - want).norm())
+        plain += float((products(g, torch.float32) - want).norm())
+    assert kernel <= bound * plain, (kernel / plain, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_orthogonalize_infinity_leaves_nothing_finite(dtype):
+    import lic_amd.functional as Fn
+    g = torch.Generator().manual_seed(11)
+    mats = [torch.randn(s, generator=g).to(dtype).to(DEV) for s in ((1, 1), (1, 9), (5, 1), (60, 90), (300, 70), (64, 64))]
+    for m in mats:
+        m[m.shape[0] // 2, m.shape[1] // 3] = float("-inf")
+    assert not any(torch.isfinite(o).any() for o in Fn.orthogonalize(mats))
