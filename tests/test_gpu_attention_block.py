@@ -176,3 +176,93 @@ def test_wnsa_with_rotary():
                 blk.rotary = None
         b = m.run(Fn.Act(x)).t
     assert torch.isfinite(a).all() and not torch.equal(a, b)
+
+
+def test_wnsa_blocks_with_rotary(monkeypatch):
+    """Each of the four window-attention blocks of Win_noShift_Attention(rotary=), in its place with the input that it
+    meets there, against its definition in 64 bits (test_block_forward's tolerance)."""
+    import lic_amd.functional as Fn
+    from lic_amd.layers import WinBasedAttention, Win_noShift_Attention
+    torch.manual_seed(0)
+    m = Win_noShift_Attention(96, 4, 8, 4, rotary=100.0).to(DEV)
+    run, seen = WinBasedAttention.run, []
+
+    def recorded(self, x, out=None, **kw):
+        assert not kw
+        before = x.nchw().permute(0, 2, 3, 1).cpu()
+        y = run(self, x, out)
+        seen.append((self, before, y.nchw().permute(0, 2, 3, 1).cpu()))
+        return y
+    monkeypatch.setattr(WinBasedAttention, "run", recorded)
+    with torch.no_grad():
+        m.run(Fn.Act(torch.randn(1, 16, 24, 96, generator=torch.Generator().manual_seed(7)).to(DEV)))
+    assert [b for b, _, _ in seen] == [m.conv_b[i] for i in (0, 2, 5, 8)]
+    for blk, x, y in seen:
+        assert blk.rotary == 100.0
+        want = _oracle(blk, x.double())
+        assert (y.double() - want).abs().max() <= 2.3e-5 * want.abs().max()
+
+
+def test_int8_linears_of_the_codec_match_64_bits(monkeypatch):
+    """Every product that the codec runs in 8 bits, with the input, shortcut and weights that it meets there, against the
+    quantised product in 64 bits (test_gpu_int8's tolerance): they are the window-attention blocks' qkv and proj, all of
+    them."""
+    import bench
+    import lic_amd.functional as Fn
+    from lic_amd.layers import Linear, WinBasedAttention
+    from tests.test_gpu_int8 import _check, _codes, _result
+    net = bench.build_net("net_ga", "fp16", 256, 1, "cpu").cuda()
+    x = bench.bench_input(1, 256, 0).cuda()
+    blocks = [b for b in net.modules() if isinstance(b, WinBasedAttention)]
+    layers = {id(m): m for b in blocks for m in (b.attn.qkv, b.attn.proj)}
+    product, run, at, calls, ran = Fn.linear_int8, Linear.run, [], [], set()
+
+    def of_layer(self, *a, **k):
+        at.append(self)
+        try:
+            return run(self, *a, **k)
+        finally:
+            at.pop()
+
+    def recorded(a, pk, out=None, **kw):
+        rows = lambda v: v.t[..., v.c0:v.c0 + v.c].reshape(-1, v.c).clone()
+        r1, before = kw.get("r1"), rows(a)
+        shortcut = rows(r1) if r1 is not None else None
+        y = product(a, pk, out, **kw)
+        ran.add(id(at[-1]))
+        calls.append((at[-1], before, shortcut, kw.get("act", 0), rows(y)))
+        return y
+    monkeypatch.setattr(Linear, "run", of_layer)
+    monkeypatch.setattr(Fn, "linear_int8", recorded)
+    with torch.no_grad(), Fn.int8_linears():
+        net(x, "test")
+    used = [b for b in blocks if id(b.attn.qkv) in ran]
+    assert len(used) >= 8 and len(calls) == 2 * len(used) and ran <= layers.keys()
+    assert ran == {id(m) for b in used for m in (b.attn.qkv, b.attn.proj)}
+    for layer, a, r1, act, y in calls:
+        assert act == 0 and y.dtype == torch.float16
+        codes, scale = _codes(a.cpu())
+        wc, ws = _codes(layer.weight.detach().cpu())
+        _check(y, *_result(codes, scale, wc, ws, layer.bias.detach().cpu().double(), 0, 0,
+                           r1.cpu().double() if r1 is not None else None))
+
+
+def test_eval_cli_with_int8_linears(capsys):
+    """eval_net.py --int8-linear: the sweep inside the context, named in its line; nothing of it stays."""
+    import json
+    import eval_net
+    import lic_amd.functional as Fn
+    args = ["--synthetic-kodak", "--lambdas", "0.0067", "--precision", "fp16", "--graph"]
+    lines = []
+    for extra in ([], ["--int8-linear"]):
+        eval_net.main(args + extra)
+        lines.append(json.loads(capsys.readouterr().out.strip().splitlines()[-1]))
+        assert not Fn.int8_mode()
+    plain, eight = lines
+    assert plain["precision"] == "fp16" and eight["precision"] == "fp16+int8_linear"
+    with Fn.int8_linears():
+        want, _, _ = eval_net.rd_sweep([0.0067], "", arch="net_ga", precision="fp16", graph=False, batched=True)
+    for key in ("bpp", "psnr", "images"):
+        assert eight["rd"][0][key] == want[0][key]
+    assert eight["rd"][0]["psnr"] != plain["rd"][0]["psnr"]
+    print("\n[int8 linears] fp16", plain["rd"], "8-bit", eight["rd"])

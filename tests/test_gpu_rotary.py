@@ -245,3 +245,24 @@ def test_rotary_more_workgroups_than_a_grid_dimension():
     torch.cuda.empty_cache()
     pos = torch.stack([at // W, at % W])[:, None, None]
     _check(got.view(1, 1, -1, 1025), *_oracle(rows.view(1, 1, -1, 1025), plan, 1, pos))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["half", "pairs"])
+@pytest.mark.parametrize("listed", [False, True])
+def test_rotary_gradient_16_bit(dtype, layout, listed):
+    """The training path's types: forward and gradient of a map with channels that pass through, a gradient that arrives
+    strided, positions of the grid and listed, against 64 bits."""
+    import lic_amd.functional as Fn
+    from lic_amd import autograd as AG
+    g = torch.Generator().manual_seed(6)
+    plan = Fn.RotaryPlan(24, (6, 6), layout=layout, device=DEV)
+    x, dy = (torch.randn(2, 8, 12, 72, generator=g).to(dtype) for _ in range(2))
+    pos = torch.randint(-5000, 5000, (2, 2, 8, 12), generator=g, dtype=torch.int32) if listed else None
+    full = pos if listed else _grid(2, 8, 12, 2)
+    leaf = x.to(DEV).requires_grad_(True)
+    y = AG.rotary(leaf, plan, 2, pos.to(DEV) if listed else None)
+    strided = dy.to(DEV).permute(0, 3, 1, 2).contiguous().permute(0, 2, 3, 1)
+    dx, = torch.autograd.grad(y, leaf, strided)
+    _check(y.detach(), *_oracle(x, plan, 2, full))
+    _check(dx, *_oracle(dy, plan, 2, full, inverse=True))
