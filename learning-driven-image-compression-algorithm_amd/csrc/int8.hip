@@ -315,9 +315,10 @@ __device__ __forceinline__ int int8_channel(int r) {
 // Tiled product: BM tokens x BN channels a workgroup of WM x WN waves, 64 bytes of k a step, four steps of both operands
 // in LDS, three of them in flight by LDS-DMA while one is multiplied (one barrier a step).  A row's four 16-byte chunks sit
 // at chunk ^ (row / 2) % 4: eight neighbouring lanes of a fragment read cover all 64 banks.  Bound by the matrix
-// instructions: 8192 x 4096 -> 8192 282 us, 1.95 POP/s (a large library product reaches 2.06); small ones by the latency of
-// their k steps, which KG groups of waves take a part of each and join in LDS: 128 x 4096 -> 4096 12.9 us with one, 9.9 with
-// two; 1037 x 333 -> 517 fp32 5.3 us.  More than four steps in flight gain nothing (128 x 4096 -> 4096 13.5 us with eight).
+// instructions: 8192 x 4096 -> 8192 282 us, 1.95 POP/s, on the same operands again and again, 300 to 318 on new ones (a large
+// library product reaches 2.06); small ones by the latency of their k steps, which KG groups of waves take a part of each and
+// join in LDS: 128 x 4096 -> 4096 12.9 us with one, 9.9 with two; 1037 x 333 -> 517 fp32 5.3 us.  More than four steps in flight
+// gain nothing (128 x 4096 -> 4096 13.5 us with eight).
 template <typename T, int BM, int BN, int WM, int WN, int KG>
 __global__ __launch_bounds__(64 * WM * WN * KG) void int8_tile_kernel(Int8Args a, int mt, int nt) {
   constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, BK = 64, STAGES = 4;
@@ -501,7 +502,7 @@ __global__ __launch_bounds__(512) void int8_few_kernel(Int8Args a) {
 }
 
 // One to ONE_TOKENS tokens of up to ONE_K channels in one launch: every workgroup quantises them into LDS, its first weights
-// already under way.  Bound by latency, then the weights' bytes: 1 x 4096 -> 4096 7.5 us (quantised apart: 5.6 + 5.4).
+// already under way.  Bound by latency, then the weights' bytes: 1 x 4096 -> 4096 7.5 to 8 us (quantised apart: 5.6 + 5.4).
 constexpr int ONE_TOKENS = 4, ONE_K = 4096;
 template <typename T>
 __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
@@ -567,8 +568,9 @@ __global__ __launch_bounds__(512) void int8_one_kernel(Int8Args a) {
 // Few tiles of up to FUSED_K channels in one launch: 32 tokens x 128 channels a workgroup.  Its weights are all asked for at
 // once (LDS-DMA), and while they come its tokens are quantised into LDS, sixteen lanes a token; then its 8 waves multiply, four
 // tiles of 32 x 32 in two halves of k that are joined in LDS.  Each of a token's tiles quantises it again.  us (two launches):
-// 64 x 192 -> 576 fp16 4.6 (5.5), 1037 x 333 -> 517 fp32 8.1 (8.4), 2500 x 192 -> 576 (395 tiles) 6.3 (7.8), fp32 8.0 (9.3),
-// 2000 x 384 -> 1000 fp32 (504) 12.7 (11.8), 4096 x 192 -> 576 (640) 7.9 (8.4), fp32 10.5 (10.8); and a call, a workspace less.
+// 64 x 192 -> 576 fp16 4.6 (5.5), 1037 x 333 -> 517 fp32 8.1 (8.4; 9.2 with an activation and a shortcut), 2500 x 192 -> 576 (395
+// tiles) 6.3 (7.8), fp32 8.0 (9.3), 2000 x 384 -> 1000 fp32 (504) 12.7 (11.8), 4096 x 192 -> 576 (640) 7.9 (8.4), fp32 10.5
+// (10.8); and a call, a workspace less.
 constexpr int FUSED_K = 384, FUSED_M = 32, FUSED_N = 128, FUSED_TILES = 512;
 constexpr int FUSED_SUMS = 4 * (4096 + 4 * INT8_STAGE);   // four tiles of sums, then four waves' staging
 template <typename T>
@@ -636,7 +638,7 @@ __global__ __launch_bounds__(512) void int8_fused_kernel(Int8Args a) {
 // Many tokens of few channels (kpad = 64 KS; whole tiles of y only: n a multiple of 32, aligned): 32 tokens a wave, quantised
 // straight into matrix operands that stay in registers; the weights pass through LDS, 64 channels at a time, the next under
 // way.  x is read once and y written once, the codes never reach memory.  Bound by the bytes of y: 131072 x 192 -> 576 fp16
-// 44 us alone, 53 with the call (201 MB; 35 without its stores).  A weight row's 16-byte chunks are placed so that a fragment
+// 42 to 48 us alone, 55 with the call (201 MB; 35 without its stores).  A weight row's 16-byte chunks are placed so that a fragment
 // read meets every bank once: rows advance by 16 KS of the 64 words, so chunk ^ swizzle(row) within 4, 8 or 16 chunks spreads
 // those that coincide.
 template <int KS>
