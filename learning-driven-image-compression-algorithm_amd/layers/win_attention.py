@@ -67,6 +67,11 @@ class WindowAttention(nn.Module):
         self.qkv.int8 = self.proj.int8 = True   # taken by functional.int8_linears
         _trunc_normal_(self.relative_position_bias_table, std=.02)
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for layer in (self.qkv, self.proj):   # of blocks stored whole before the layers had it
+            layer.__dict__.setdefault("int8", True)
+
 
 class WinBasedAttention(nn.Module):
     """``rotary``: a base (e.g. 100.0) turns q and k by their token's row and column before the scores, half of a

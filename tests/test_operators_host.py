@@ -522,3 +522,14 @@ def test_c_entries_refuse_what_no_launch_takes():
         return lib.lic_orthogonalize_workspace(0, count, m)
     assert tiles(64, 2 ** 24) > 0 and tiles(64 * 63, 2 ** 24) > 0     # 63 * 2^18 tiles
     assert tiles(64 * 64, 2 ** 24) == -1 and tiles(64, 2 ** 24, 64) == -1
+
+
+def test_int8_scope_of_blocks_stored_whole():
+    """Blocks pickled as modules before the layers had the attribute are taken as new ones are; a choice made is kept."""
+    import pickle
+    from lic_amd.layers import WinBasedAttention
+    blk = WinBasedAttention(32, 4, 8)
+    del blk.attn.qkv.__dict__["int8"]
+    blk.attn.proj.int8 = False
+    old = pickle.loads(pickle.dumps(blk))
+    assert old.attn.qkv.int8 is True and old.attn.proj.int8 is False
