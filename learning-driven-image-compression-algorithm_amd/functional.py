@@ -1082,7 +1082,7 @@ def _on_current_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
 
 def _in_32_bits(what: str, *sizes: int) -> None:
     """The C entries' sizes have 32 bits, and ctypes cuts longer ones off without a word."""
-    if max(sizes) >= 1 << 31:
+    if max(sizes, default=0) >= 1 << 31:
         raise ValueError(f"{what}: sizes of 2^31 and more are out of range")
 
 
@@ -1344,7 +1344,7 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs: Sequence
     for g in mats:
         if g.dim() != 2 or g.dtype != dt:
             raise ValueError("orthogonalize: a list of 2-D matrices of one dtype")
-    _in_32_bits("orthogonalize", *(n for g in mats for n in g.shape))
+    _in_32_bits("orthogonalize", *(n for g in mats if g.numel() for n in g.shape))
     _on_current_device("orthogonalize", *mats)
     if len(coeffs) != 3 or not all(math.isfinite(c) for c in coeffs):
         raise ValueError("orthogonalize: coeffs = (a, b, c), finite")

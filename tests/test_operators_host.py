@@ -533,3 +533,9 @@ def test_int8_scope_of_blocks_stored_whole():
     blk.attn.proj.int8 = False
     old = pickle.loads(pickle.dumps(blk))
     assert old.attn.qkv.int8 is True and old.attn.proj.int8 is False
+
+
+def test_long_empty_matrices_are_not_refused_for_their_length():
+    """An empty matrix has nothing to compute, however long its other side is."""
+    with pytest.raises(ValueError, match="not on the GPU"):   # the next check
+        Fn.orthogonalize([torch.empty(0, 2 ** 32 + 1)])
